@@ -289,7 +289,7 @@ def _own_pool(st):
         ab.kv_copy_pages(st["arrays"], st["KV"] * PAGE * st["hd"], st["pages"], st["src"], st["dst"], st["n"], stream=stream)
     else:
         ab.kv_compact(st["arrays"], st["pages"], st["KV"], st["hd"], st["table"], st["stride"], st["base"], st["keep"],
-                      st["start"], st["S"], stream=stream)
+                      st["start"], st["S"], st["kept"], stream=stream)
     return st["pool"]
 
 
