@@ -212,6 +212,96 @@ int aaedn_cu_attention_noalloc(const float* d_q, const float* d_k, const float* 
                                size_t num_segments, float* d_out, size_t n_heads, size_t head_dim, float scale,
                                void* stream);
 
+/* ---- operators of a batched step ------------------------------------------
+ * No counterpart in the reference (its token loop runs one token of one
+ * sequence). They work on a paged cache in the layout of the batched model
+ * below: pools of pages of AAEDN_KV_PAGE_TOKENS tokens and a table of page
+ * numbers per sequence. Index arrays are read on the device, so a captured
+ * call can be replayed after they changed; whatever they hold, nothing
+ * outside the given arrays is read or written. */
+#define AAEDN_KV_PAGE_TOKENS 64
+typedef struct {
+    const float *d_k, *d_v;      /* [n_pages][n_kv_heads][64][head_dim] fp32 */
+    const int32_t* d_page_table; /* [n_seqs][pt_stride]: token t of sequence s is row t % 64 of page
+                                  * d_page_table[s * pt_stride + t / 64] */
+    size_t pt_stride;
+    uint32_t n_pages, n_kv_heads, head_dim;
+} aaedn_kv_cache;
+
+/* Attention of packed query rows: the new tokens of n_seqs sequences in one
+ * call (whole prompts, continued chats, single tokens, of different lengths).
+ * Sequence s owns rows d_row_start[s] .. d_row_start[s + 1] - 1 of d_q and
+ * d_out ([rows][ldq / ldo], n_heads * head_dim floats of each used; ascending
+ * d_row_start); its row r is the token in cache slot d_past[s] + r, whose K
+ * and V are in the cache already, and attends slots 0 .. d_past[s] + r. Query
+ * head h reads K/V head h / (n_heads / n_kv_heads). out = softmax(scale *
+ * q k^T) v with the softmax and all sums in fp32; the products are fp32
+ * accurate (2^-22 of each factor and 2^-38 of the largest K or V value of the
+ * same page and head). Rows that no sequence owns keep their contents. Keys
+ * in pages outside 0 .. n_pages - 1 or behind the table are left out; a row
+ * with no key left gives zeros; NaN and infinities in slots that a row does
+ * not attend have no effect on it, and a row that attends one is NaN.
+ * head_dim a multiple of 4 up to 256 (the tensor-core path takes up to 128),
+ * n_heads / n_kv_heads up to 64, d_q, d_k, d_v, d_out and the workspace
+ * 16-byte aligned, ldq and ldo multiples of 4. d_workspace:
+ * AAEDN_ATTN_ROWS_WORKSPACE_BYTES of scratch, which needs no
+ * initialisation and holds nothing between calls; calls (and captured graphs)
+ * that can overlap on the GPU need one each. A bounded device wait that ran
+ * out is reported by aaedn_device_sync. */
+#define AAEDN_ATTN_ROWS_WORKSPACE_BYTES (32u << 20)
+int aaedn_cu_attention_packed(const float* d_q, size_t ldq, const aaedn_kv_cache* cache, const int32_t* d_row_start,
+                              const int32_t* d_past, size_t n_seqs, size_t rows, size_t n_heads, float scale,
+                              float* d_out, size_t ldo, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The same for trees of drafted tokens: sequence s has d_past[s] cached tokens
+ * and its rows are nodes, node j in slot d_past[s] + j. A row attends the
+ * d_past[s] cached tokens and the nodes whose bit is set in its mask: bit
+ * j % 64 of word j / 64 of d_mask ([rows][mask_words]; a node's own bit and
+ * its ancestors' for a tree, but any mask is taken; bits of nodes that the
+ * sequence does not have are ignored). */
+int aaedn_cu_attention_tree(const float* d_q, size_t ldq, const aaedn_kv_cache* cache, const int32_t* d_row_start,
+                            const int32_t* d_past, const uint64_t* d_mask, size_t mask_words, size_t n_seqs,
+                            size_t rows, size_t n_heads, float scale, float* d_out, size_t ldo, void* d_workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Page copies (copy on write of forked sequences): page d_dst[i] = page
+ * d_src[i], i < n, in each of the n_arrays pools h_arrays (host array of
+ * device pointers, for example K and V of every layer; at most 4096) of
+ * n_pages pages of page_floats floats (a multiple of 4). All copies run at
+ * once: no page may be a destination twice, or a destination and a source.
+ * Pairs with a page number outside 0 .. n_pages - 1 are skipped. */
+int aaedn_cu_kv_copy_pages(float* const* h_arrays, size_t n_arrays, size_t page_floats, uint32_t n_pages,
+                           const int32_t* d_src, const int32_t* d_dst, size_t n, void* stream);
+
+/* Compaction after a verified draft: for sequence s and i < d_keep_start[s +
+ * 1] - d_keep_start[s], the row of slot d_base[s] + i becomes what slot
+ * d_base[s] + d_keep[d_keep_start[s] + i] held, in each of the n_arrays pools
+ * ([n_pages][n_kv_heads][64][head_dim]). Each sequence's keep list is
+ * strictly ascending from 0 up, n_keep entries in all (the length of d_keep); the sequences' slots lie in different pages
+ * or do not overlap. Entries with a slot outside the table or a page outside
+ * the pool are skipped. */
+int aaedn_cu_kv_compact(float* const* h_arrays, size_t n_arrays, uint32_t n_pages, uint32_t n_kv_heads,
+                        uint32_t head_dim, const int32_t* d_page_table, size_t pt_stride, const int32_t* d_base,
+                        const int32_t* d_keep, const int32_t* d_keep_start, size_t n_seqs, size_t n_keep,
+                        void* stream);
+
+/* Next tokens of many rows of logits ([rows][ld], vocab of each used, vocab up
+ * to 1000000): aaedn_cu_sample's order of the vocabulary (logit descending,
+ * ties by the lower id) with top-k and min-p, per-row parameters and fp64
+ * probabilities. With p_i = exp((l_i - max) / T), the kept tokens are the
+ * first top_k of the order, of those the ones with p_i >= min_p (so min_p is
+ * relative to the most likely token), of those up to and including the first
+ * whose cumulative mass reaches top_p times their mass; the token is the first
+ * kept one whose cumulative mass reaches u times the kept mass. Device arrays
+ * [rows]: d_temperature (null: 1; <= 0 or NaN: greedy, the lowest id of the
+ * largest logit), d_top_k (null, <= 0 or >= vocab: off), d_top_p (null or >= 1:
+ * off; <= 0: only the first token), d_min_p (null or <= 0: off; above 1 as 1),
+ * d_u (uniforms in [0, 1); others are clamped). NaN logits are never drawn; a
+ * row whose largest logit is infinite gives its lowest id, a row of NaN 0. */
+int aaedn_cu_sample_rows(const float* d_logits, size_t ld, size_t rows, uint32_t vocab, const float* d_temperature,
+                         const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, const float* d_u,
+                         uint32_t* d_tokens, void* stream);
+
 /* ---- the token loop ------------------------------------------------------
  * include/transformer.hpp:15-44 Transformer / transformer_init /
  * transformer_forward. One model owns one device arena (a single
@@ -412,6 +502,46 @@ int aaedn_seq_prefill(aaedn_model* m, uint32_t seq, const uint32_t* h_tokens, si
  * and greedy token. Synchronises. */
 int aaedn_model_step_batch(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_tokens, size_t n,
                            float* h_logits, uint32_t* h_next);
+
+/* ---- batched steps with sampling, packed prompts and drafted trees --------
+ * Host arrays, one entry per row of the call: temperature, top_k, top_p,
+ * min_p as d_temperature, d_top_k, d_top_p, d_min_p of aaedn_cu_sample_rows
+ * (each may be null) and the uniforms (required). A null aaedn_sampling* is
+ * greedy. */
+typedef struct {
+    const float* h_temperature;
+    const int32_t* h_top_k;
+    const float *h_top_p, *h_min_p, *h_u;
+} aaedn_sampling;
+/* aaedn_model_step_batch with each row's next token drawn on the device. */
+int aaedn_model_step_sample(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_tokens, size_t n,
+                            const aaedn_sampling* sampling, float* h_logits, uint32_t* h_next);
+/* aaedn_seq_prefill of n distinct sequences at once: h_counts[i] >= 1 tokens
+ * of sequence h_seqs[i], concatenated in h_tokens, packed into common passes
+ * of aaedn_model_prefill_rows tokens (attention: aaedn_cu_attention_packed);
+ * h_logits [n][vocab] and h_next [n] (either may be null) receive each
+ * sequence's last logits and next token. Synchronises. */
+int aaedn_seq_prefill_batch(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts,
+                            const uint32_t* h_tokens, size_t n, const aaedn_sampling* sampling, float* h_logits,
+                            uint32_t* h_next);
+/* Verification of drafted trees: for each of n distinct sequences h_counts[i]
+ * (1..256, aaedn_model_prefill_rows in all) nodes with tokens h_tokens and
+ * parents h_parents (concatenated; the parent is an earlier node of the same
+ * sequence, -1: the sequence's last token), all in one pass
+ * (aaedn_cu_attention_tree). h_logits [nodes][vocab] and h_next [nodes]
+ * (either may be null) receive what follows each node. The sequences keep
+ * their lengths; aaedn_seq_accept then takes the nodes to keep. Any other
+ * call on a sequence drops its draft. Synchronises. */
+int aaedn_model_step_tree(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts, const uint32_t* h_tokens,
+                          const int32_t* h_parents, size_t n, const aaedn_sampling* sampling, float* h_logits,
+                          uint32_t* h_next);
+/* Appends to each sequence the h_counts[i] (possibly 0) nodes of its last
+ * drafted tree listed in h_nodes (concatenated): a path from the sequence's
+ * last token, every node the child of the one before. Their K/V rows move to
+ * the sequence's next slots (aaedn_cu_kv_compact) and the rest of the draft is
+ * dropped, its pages given back. AAEDN_ESTATE without a drafted tree. */
+int aaedn_seq_accept(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts, const uint32_t* h_nodes,
+                     size_t n);
 
 #ifdef __cplusplus
 }

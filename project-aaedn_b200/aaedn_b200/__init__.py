@@ -49,6 +49,19 @@ class AbnHeader(ctypes.Structure):
                 ("ffn_dim", _u32), ("quant_type", ctypes.c_uint8)]
 
 
+KV_PAGE_TOKENS = 64
+ATTN_ROWS_WORKSPACE_BYTES = 32 << 20
+
+
+class KvCacheView(ctypes.Structure):
+    _fields_ = [("d_k", _vp), ("d_v", _vp), ("d_page_table", _vp), ("pt_stride", _sz), ("n_pages", _u32),
+                ("n_kv_heads", _u32), ("head_dim", _u32)]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [("h_temperature", _vp), ("h_top_k", _vp), ("h_top_p", _vp), ("h_min_p", _vp), ("h_u", _vp)]
+
+
 class TpPlan(ctypes.Structure):
     _fields_ = [(n, _u32) for n in ("n_heads", "n_kv_heads", "ffn_dim", "vocab", "q_head0", "kv_head0",
                                     "ffn_row0", "vocab0", "o_k", "down_k")]
@@ -112,6 +125,13 @@ def lib():
         "aaedn_cu_ffn_swiglu": ([_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp], _int),
         "aaedn_memcpy_d2d": ([_vp, _vp, _sz, _vp], _int),
         "aaedn_cu_sample": ([_vp, _u32, ctypes.c_float, ctypes.c_float, ctypes.c_float, _vp, _vp], _int),
+        "aaedn_cu_attention_packed": ([_vp, _sz, ctypes.POINTER(KvCacheView), _vp, _vp, _sz, _sz, _sz, _f32, _vp, _sz,
+                                       _vp, _sz, _vp], _int),
+        "aaedn_cu_attention_tree": ([_vp, _sz, ctypes.POINTER(KvCacheView), _vp, _vp, _vp, _sz, _sz, _sz, _sz, _f32,
+                                     _vp, _sz, _vp, _sz, _vp], _int),
+        "aaedn_cu_kv_copy_pages": ([_vp, _sz, _sz, _u32, _vp, _vp, _sz, _vp], _int),
+        "aaedn_cu_kv_compact": ([_vp, _sz, _u32, _u32, _u32, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _vp], _int),
+        "aaedn_cu_sample_rows": ([_vp, _sz, _sz, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _int),
         "aaedn_abn_read_header": ([ctypes.c_char_p, ctypes.POINTER(AbnHeader)], _int),
         "aaedn_abn_read_payload": ([ctypes.c_char_p, ctypes.POINTER(AbnHeader), _vp, _vp], _int),
         "aaedn_model_create": ([ctypes.POINTER(ModelConfig), ctypes.POINTER(_vp)], _int),
@@ -148,6 +168,10 @@ def lib():
         "aaedn_model_kv_pages": ([_vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32)], _int),
         "aaedn_seq_prefill": ([_vp, _u32, _vp, _sz, _vp, _vp], _int),
         "aaedn_model_step_batch": ([_vp, _vp, _vp, _sz, _vp, _vp], _int),
+        "aaedn_model_step_sample": ([_vp, _vp, _vp, _sz, ctypes.POINTER(Sampling), _vp, _vp], _int),
+        "aaedn_seq_prefill_batch": ([_vp, _vp, _vp, _vp, _sz, ctypes.POINTER(Sampling), _vp, _vp], _int),
+        "aaedn_model_step_tree": ([_vp, _vp, _vp, _vp, _vp, _sz, ctypes.POINTER(Sampling), _vp, _vp], _int),
+        "aaedn_seq_accept": ([_vp, _vp, _vp, _vp, _sz], _int),
         "aaedn_model_logits": ([_vp, _vp], _int),
         "aaedn_model_tokens": ([_vp, _vp, _sz], _int),
         "aaedn_model_forward_debug": ([_vp, _u32, _vp, _vp], _int),
@@ -328,6 +352,85 @@ def attention_noalloc(d_q, d_k, d_v, segments, d_out, n_heads, head_dim, scale, 
 
 
 ATTN_NOALLOC_SCRATCH_BYTES = 1 << 20
+
+
+# ---------------------------------------------- operators of a batched step
+class KvCache:
+    """A paged K/V cache as the batched operators read it (aaedn_kv_cache):
+    pools [n_pages][n_kv_heads][64][head_dim] and the table of page numbers
+    [n_seqs][pt_stride], all on the device. Keeps what it was given alive."""
+
+    def __init__(self, d_k, d_v, d_page_table, pt_stride, n_pages, n_kv_heads, head_dim):
+        self._keep = (d_k, d_v, d_page_table)
+        self.head_dim = int(head_dim)
+        self.view = KvCacheView(_p(d_k), _p(d_v), _p(d_page_table), pt_stride, n_pages, n_kv_heads, head_dim)
+        self.ref = ctypes.byref(self.view)
+
+
+def attention_packed(d_q, cache, d_row_start, d_past, n_seqs, rows, n_heads, scale, d_out, d_workspace,
+                     workspace_bytes=ATTN_ROWS_WORKSPACE_BYTES, ldq=None, ldo=None, stream=None):
+    """Causal attention of the new tokens of several sequences over their
+    cached pages (aaedn_cu_attention_packed): rows d_row_start[s].. of d_q are
+    the tokens at positions d_past[s].. of sequence s."""
+    n = n_heads * cache.head_dim
+    check(lib().aaedn_cu_attention_packed(_p(d_q), ldq or n, cache.ref, _p(d_row_start), _p(d_past), n_seqs, rows,
+                                          n_heads, scale, _p(d_out), ldo or n, _p(d_workspace), workspace_bytes,
+                                          stream))
+
+
+def attention_tree(d_q, cache, d_row_start, d_past, d_mask, mask_words, n_seqs, rows, n_heads, scale, d_out,
+                   d_workspace, workspace_bytes=ATTN_ROWS_WORKSPACE_BYTES, ldq=None, ldo=None, stream=None):
+    """The same for trees of drafted tokens (aaedn_cu_attention_tree): a row
+    attends its sequence's cached tokens and the nodes of its mask."""
+    n = n_heads * cache.head_dim
+    check(lib().aaedn_cu_attention_tree(_p(d_q), ldq or n, cache.ref, _p(d_row_start), _p(d_past), _p(d_mask),
+                                        mask_words, n_seqs, rows, n_heads, scale, _p(d_out), ldo or n,
+                                        _p(d_workspace), workspace_bytes, stream))
+
+
+def tree_masks(parents):
+    """The mask words of a drafted tree: parents[i] < i is the node that node i
+    follows (-1: the last cached token); uint64 [n][ceil(n / 64)], a node's own
+    bit and its ancestors'."""
+    n = len(parents)
+    words = np.zeros((n, max(1, (n + 63) // 64)), np.uint64)
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"parents[{i}] = {p} is not -1 or an earlier node")
+        if p >= 0:
+            words[i] = words[p]
+        words[i, i >> 6] |= np.uint64(1 << (i & 63))
+    return words
+
+
+def _arrays(d_arrays):
+    """A host array of device pointers (pass one made earlier as it is)."""
+    if isinstance(d_arrays, ctypes.Array):
+        return d_arrays
+    return (_vp * len(d_arrays))(*[_p(a) for a in d_arrays])
+
+
+def kv_copy_pages(d_arrays, page_floats, n_pages, d_src, d_dst, n, stream=None):
+    """Page d_dst[i] = page d_src[i] in every pool of d_arrays
+    (aaedn_cu_kv_copy_pages)."""
+    arr = _arrays(d_arrays)
+    check(lib().aaedn_cu_kv_copy_pages(arr, len(arr), page_floats, n_pages, _p(d_src), _p(d_dst), n, stream))
+
+
+def kv_compact(d_arrays, n_pages, n_kv_heads, head_dim, d_page_table, pt_stride, d_base, d_keep, d_keep_start, n_seqs,
+               n_keep, stream=None):
+    """Slots d_base[s] + keep of every pool moved to d_base[s] + 0, 1, ...
+    (aaedn_cu_kv_compact)."""
+    arr = _arrays(d_arrays)
+    check(lib().aaedn_cu_kv_compact(arr, len(arr), n_pages, n_kv_heads, head_dim, _p(d_page_table), pt_stride,
+                                    _p(d_base), _p(d_keep), _p(d_keep_start), n_seqs, n_keep, stream))
+
+
+def sample_rows(d_logits, rows, vocab, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_tokens, ld=None, stream=None):
+    """Next tokens of many rows of logits (aaedn_cu_sample_rows): per-row
+    temperature, top-k, top-p, min-p (None: off) and uniforms."""
+    check(lib().aaedn_cu_sample_rows(_p(d_logits), ld or vocab, rows, vocab, _p(d_temperature), _p(d_top_k),
+                                     _p(d_top_p), _p(d_min_p), _p(d_u), _p(d_tokens), stream))
 
 
 def device_sync():
@@ -622,3 +725,73 @@ class BatchedModel(Model):
         nxt = np.zeros(sq.size, np.uint32)
         check(lib().aaedn_model_step_batch(self.h, _p(sq), _p(t), sq.size, _p(logits), _p(nxt)))
         return logits, nxt
+
+    def _sampling(self, n, sampling):
+        """sampling: None (greedy) or a dict with u and any of temperature,
+        top_k, top_p, min_p, each one value or one per row."""
+        if sampling is None:
+            return None, None
+        unknown = set(sampling) - {"temperature", "top_k", "top_p", "min_p", "u"}
+        if unknown or "u" not in sampling:
+            raise ValueError(f"sampling takes u and temperature, top_k, top_p, min_p: got {sorted(sampling)}")
+        kept = {k: np.ascontiguousarray(np.broadcast_to(np.asarray(v, np.int32 if k == "top_k" else np.float32), (n,)))
+                for k, v in sampling.items()}
+        s = Sampling(**{"h_" + k: v.ctypes.data for k, v in kept.items()})
+        return ctypes.byref(s), (s, kept)
+
+    def step_sample(self, seqs, tokens, sampling, want_logits=False):
+        """step() with each row's next token drawn on the device
+        (aaedn_model_step_sample); (logits or None, next [n])."""
+        sq = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        t = np.ascontiguousarray(tokens, np.uint32).reshape(-1)
+        if t.size != sq.size:
+            raise ValueError("one token per sequence")
+        ref, keep = self._sampling(sq.size, sampling)
+        logits = np.empty((sq.size, self.cfg["vocab"]), np.float32) if want_logits else None
+        nxt = np.zeros(sq.size, np.uint32)
+        check(lib().aaedn_model_step_sample(self.h, _p(sq), _p(t), sq.size, ref, _p(logits), _p(nxt)))
+        return logits, nxt
+
+    @staticmethod
+    def _ragged(lists, dtype):
+        rows = [np.ascontiguousarray(x, dtype).reshape(-1) for x in lists]
+        counts = np.array([r.size for r in rows], np.uint32)
+        return counts, np.concatenate(rows) if rows else np.empty(0, dtype)
+
+    def prefill_batch(self, seqs, tokens, sampling=None, want_logits=True):
+        """Appends tokens[i] (a list) to sequence seqs[i], all in common passes
+        (aaedn_seq_prefill_batch); (last logits [n][vocab] or None, next [n])."""
+        sq = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        counts, flat = self._ragged(tokens, np.uint32)
+        if counts.size != sq.size:
+            raise ValueError("one token list per sequence")
+        ref, keep = self._sampling(sq.size, sampling)
+        logits = np.empty((sq.size, self.cfg["vocab"]), np.float32) if want_logits else None
+        nxt = np.zeros(sq.size, np.uint32)
+        check(lib().aaedn_seq_prefill_batch(self.h, _p(sq), _p(counts), _p(flat), sq.size, ref, _p(logits), _p(nxt)))
+        return logits, nxt
+
+    def step_tree(self, seqs, tokens, parents, sampling=None, want_logits=True):
+        """Verifies one drafted tree per sequence (aaedn_model_step_tree):
+        tokens[i] and parents[i] list its nodes; (logits [nodes][vocab] or
+        None, what follows each node [nodes]), the trees concatenated."""
+        sq = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        counts, flat = self._ragged(tokens, np.uint32)
+        pcounts, par = self._ragged(parents, np.int32)
+        if counts.size != sq.size or not np.array_equal(counts, pcounts):
+            raise ValueError("one token list and one parent list of the same length per sequence")
+        ref, keep = self._sampling(flat.size, sampling)
+        logits = np.empty((flat.size, self.cfg["vocab"]), np.float32) if want_logits else None
+        nxt = np.zeros(flat.size, np.uint32)
+        check(lib().aaedn_model_step_tree(self.h, _p(sq), _p(counts), _p(flat), _p(par), sq.size, ref, _p(logits),
+                                          _p(nxt)))
+        return logits, nxt
+
+    def accept(self, seqs, nodes):
+        """Appends the path nodes[i] of its drafted tree to sequence seqs[i]
+        (aaedn_seq_accept)."""
+        sq = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        counts, flat = self._ragged(nodes, np.uint32)
+        if counts.size != sq.size:
+            raise ValueError("one node list per sequence")
+        check(lib().aaedn_seq_accept(self.h, _p(sq), _p(counts), _p(flat), sq.size))

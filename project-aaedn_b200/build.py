@@ -23,7 +23,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 INCS = ["-I" + os.path.join(ROOT, "include"), "-I" + HOST, "-I" + os.path.join(HOST, "include")]
 
-CU_SRCS = ["api.cu", "model.cu", "ffn.cu", "sample.cu", "gemm_tc.cu"]
+CU_SRCS = ["api.cu", "model.cu", "ffn.cu", "sample.cu", "gemm_tc.cu", "attn_rows.cu", "kv_pages.cu",
+           "sample_rows.cu"]
 CPP_SRCS = ["errors.cpp", "quant_tools.cpp", "abn_file.cpp", "aaedn_api.cpp", "tokenizer.cpp"]
 
 

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "attention.cuh"
+#include "attn_rows.h"
 #include "gemm_tc.h"
 #include "gemv_q4.cuh"
 
@@ -235,7 +236,9 @@ extern "C" int aaedn_stream_sync(void* stream)
 extern "C" int aaedn_device_sync(void)
 {
     AAEDN_CUDA_TRY(cudaDeviceSynchronize());
-    return tc_api_err_check();
+    if (int rc = tc_api_err_check())
+        return rc;
+    return attn_rows_err_check();
 }
 
 extern "C" int aaedn_cu_dequant_4bit(const uint8_t* d_data, const uint16_t* d_scales, float* d_out, size_t n,

@@ -1,0 +1,250 @@
+// attn_rows.cu — attention of packed query rows over the paged fp32 K/V cache
+// (the sequences of a batch in one call), causal or under a tree mask, and
+// its C ABI.
+#include <climits>
+
+#include "common.cuh"
+
+#include "attn_rows.h"
+#include "device_check.hpp"
+
+namespace aaedn_dev
+{
+
+// Set when a bounded wait of a call without its own error word ran out (an
+// array of the module: no allocation, so a first call can be captured).
+__device__ unsigned g_attn_rows_err;
+
+int attn_rows_err_check()
+{
+    unsigned e = 0;
+    AAEDN_CUDA_TRY(cudaMemcpyFromSymbol(&e, g_attn_rows_err, sizeof e));
+    if (!e)
+        return AAEDN_OK;
+    const unsigned zero = 0;
+    AAEDN_CUDA_TRY(cudaMemcpyToSymbol(g_attn_rows_err, &zero, sizeof zero));
+    return set_error(AAEDN_ETIMEOUT, "a bounded wait of a packed or tree attention ran out");
+}
+
+// The sequence of packed row r: the s with row_start[s] <= r <
+// row_start[s + 1], or -1 (a row that belongs to no sequence).
+__device__ __forceinline__ int rows_seq_of(const AttnRowsArgs& a, int r)
+{
+    int lo = 0, hi = a.n_seqs; // first s with row_start[s + 1] > r
+    while (lo < hi)
+    {
+        const int mid = (lo + hi) >> 1;
+        if (a.row_start[mid + 1] > r)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return lo < a.n_seqs && a.row_start[lo] <= r ? lo : -1;
+}
+
+__device__ __forceinline__ const int* rows_page_table(const AttnRowsArgs& a, int s)
+{
+    return a.page_table + (size_t)(a.seq_of ? a.seq_of[s] : s) * a.pt_stride;
+}
+
+// ---------------------------------------------------------------------------
+// One warp per (packed row, query head), every head_dim (a multiple of 4, at
+// most 256). Keys come 32 at a time: lane j scores key s0 + j against q (in
+// shared memory), the softmax is carried online (running max and sum), then
+// the lanes take the head dims and add the keys' weighted V rows. fp32
+// throughout; a key that the row may not attend is never read, so what such
+// a slot holds (NaN, an unused page) has no effect. A row with no key gives
+// zeros.
+// ---------------------------------------------------------------------------
+constexpr int RW_WARPS = 4;
+
+template <bool TREE>
+__global__ void __launch_bounds__(RW_WARPS * 32) attn_rows_warp_kernel(const AttnRowsArgs a)
+{
+    __shared__ __align__(16) float qs[RW_WARPS][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.x * RW_WARPS + warp, h = blockIdx.y;
+    if (row >= a.rows)
+        return;
+    const int s = rows_seq_of(a, row);
+    if (s < 0)
+        return;
+    const int hd = a.head_dim, kvh = h / (a.n_heads / a.n_kv);
+    const float* qr = a.q + (size_t)row * a.ldq + (size_t)h * hd;
+    for (int d = lane; d < hd; d += 32)
+        qs[warp][d] = qr[d];
+    __syncwarp();
+    const long long past = max(a.past[s], 0), cap = (long long)a.pt_stride * ROWS_PAGE;
+    const long long local = (long long)row - a.row_start[s];
+    // keys 0..nk-1 are looked at
+    const long long nk = min(cap, TREE ? past + min((long long)a.mask_words * 64,
+                                                    (long long)min(a.row_start[s + 1], a.rows) - a.row_start[s])
+                                       : past + local + 1);
+    const int* pt = rows_page_table(a, s);
+    const uint64_t* mask = TREE ? a.mask + (size_t)row * a.mask_words : nullptr;
+    auto kv_at = [&](const float* base, long long key) -> const float* {
+        const int page = pt[key / ROWS_PAGE];
+        if (page < 0 || page >= a.n_pages)
+            return nullptr; // not a page: as a masked key
+        return base + (((size_t)page * a.n_kv + kvh) * ROWS_PAGE + (size_t)(key % ROWS_PAGE)) * hd;
+    };
+    auto seen = [&](long long key) {
+        if (!TREE || key < past)
+            return true;
+        const int j = (int)(key - past);
+        return ((mask[j >> 6] >> (j & 63)) & 1) != 0;
+    };
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float mrun = -INFINITY, lrun = 0.0f;
+    for (long long s0 = 0; s0 < nk; s0 += 32)
+    {
+        const long long key = s0 + lane;
+        const float* kr = key < nk && seen(key) ? kv_at(a.k, key) : nullptr;
+        float sc = -INFINITY;
+        if (kr)
+        {
+            float dot = 0.0f;
+            for (int c = 0; c < (hd >> 2); ++c)
+            {
+                const float4 kv = reinterpret_cast<const float4*>(kr)[c];
+                const float4 qv = reinterpret_cast<const float4*>(qs[warp])[c];
+                dot = fmaf(qv.x, kv.x, dot);
+                dot = fmaf(qv.y, kv.y, dot);
+                dot = fmaf(qv.z, kv.z, dot);
+                dot = fmaf(qv.w, kv.w, dot);
+            }
+            sc = dot * a.scale;
+        }
+        const float mnew = fmaxf(mrun, warp_max(sc));
+        const float ref = mnew == -INFINITY ? 0.0f : mnew; // nothing attended so far
+        const float w = kr ? expf(sc - ref) : 0.0f;
+        const float corr = expf(mrun - ref);
+        lrun = lrun * corr + warp_sum(w);
+        mrun = mnew;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            acc[i] *= corr;
+        const unsigned live = __ballot_sync(0xffffffffu, kr != nullptr);
+        for (int j = 0; j < 32; ++j)
+        {
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (!((live >> j) & 1))
+                continue;
+            const float* vr = kv_at(a.v, s0 + j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 32 * i < hd)
+                    acc[i] = fmaf(wj, vr[lane + 32 * i], acc[i]);
+        }
+    }
+    const float inv = lrun == 0.0f ? 0.0f : 1.0f / lrun;
+    float* o = a.out + (size_t)row * a.ldo + (size_t)h * hd;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < hd)
+            o[lane + 32 * i] = acc[i] * inv;
+}
+
+int attn_rows_init() { return AAEDN_OK; }
+
+int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
+{
+    const dim3 grid((unsigned)((a.rows + RW_WARPS - 1) / RW_WARPS), (unsigned)a.n_heads);
+    if (a.mask)
+        attn_rows_warp_kernel<true><<<grid, RW_WARPS * 32, 0, st>>>(a);
+    else
+        attn_rows_warp_kernel<false><<<grid, RW_WARPS * 32, 0, st>>>(a);
+    AAEDN_LAUNCH_CHECK("attn_rows_warp_kernel");
+    return AAEDN_OK;
+}
+
+} // namespace aaedn_dev
+
+using namespace aaedn_dev;
+
+namespace
+{
+
+int rows_call(const char* fn, bool tree, const float* d_q, size_t ldq, const aaedn_kv_cache* cache,
+              const int32_t* d_row_start, const int32_t* d_past, const uint64_t* d_mask, size_t mask_words,
+              size_t n_seqs, size_t rows, size_t n_heads, float scale, float* d_out, size_t ldo, void* d_workspace,
+              size_t workspace_bytes, void* stream)
+{
+    if (n_seqs == 0 || rows == 0)
+        return AAEDN_OK;
+    if (!cache)
+        return set_error(AAEDN_EINVAL, "%s: cache is null", fn);
+    const aaedn_kv_cache& c = *cache;
+    const size_t hd = c.head_dim;
+    if (hd == 0 || hd % 4 || hd > 256)
+        return set_error(AAEDN_EINVAL, "%s: head_dim %zu is not a multiple of 4 in 4..256", fn, hd);
+    if (c.n_kv_heads == 0 || n_heads == 0 || n_heads % c.n_kv_heads || n_heads / c.n_kv_heads > 64 || n_heads > 65535)
+        return set_error(AAEDN_EINVAL, "%s: n_heads %zu must be n_kv_heads (%u) times 1..64, at most 65535", fn, n_heads,
+                         c.n_kv_heads);
+    if (n_seqs > 65536 || rows > (size_t)(1 << 24))
+        return set_error(AAEDN_EINVAL, "%s: at most 65536 sequences and 2^24 rows (%zu, %zu)", fn, n_seqs, rows);
+    if (c.n_pages == 0 || c.n_pages > (uint32_t)INT_MAX || c.pt_stride == 0 || c.pt_stride > (size_t)(1 << 24))
+        return set_error(AAEDN_EINVAL, "%s: n_pages %u and pt_stride %zu must be at least 1 (pt_stride at most 2^24)", fn,
+                         c.n_pages, c.pt_stride);
+    if (ldq < n_heads * hd || ldo < n_heads * hd || ldq % 4 || ldo % 4)
+        return set_error(AAEDN_EINVAL, "%s: ldq %zu and ldo %zu must be multiples of 4 of at least n_heads * head_dim", fn,
+                         ldq, ldo);
+    if (tree && (mask_words == 0 || mask_words > 1024))
+        return set_error(AAEDN_EINVAL, "%s: mask_words %zu outside 1..1024", fn, mask_words);
+    if (!isfinite(scale))
+        return set_error(AAEDN_EINVAL, "%s: scale is not finite", fn);
+    int rc;
+    if ((rc = check_device_ptr(fn, d_q, "d_q", 16)) || (rc = check_device_ptr(fn, c.d_k, "d_k", 16)) ||
+        (rc = check_device_ptr(fn, c.d_v, "d_v", 16)) || (rc = check_device_ptr(fn, c.d_page_table, "d_page_table", 4)) ||
+        (rc = check_device_ptr(fn, d_row_start, "d_row_start", 4)) || (rc = check_device_ptr(fn, d_past, "the cached lengths", 4)) ||
+        (rc = check_device_ptr(fn, d_out, "d_out", 16)) || (rc = check_device_ptr(fn, d_workspace, "d_workspace", 16)))
+        return rc;
+    if (tree && (rc = check_device_ptr(fn, d_mask, "d_mask", 8)))
+        return rc;
+    if (workspace_bytes < AAEDN_ATTN_ROWS_WORKSPACE_BYTES)
+        return set_error(AAEDN_EINVAL, "%s: workspace of %zu bytes, %u needed", fn, workspace_bytes,
+                         AAEDN_ATTN_ROWS_WORKSPACE_BYTES);
+    AttnRowsArgs a{};
+    a.q = d_q;
+    a.ldq = ldq;
+    a.k = c.d_k;
+    a.v = c.d_v;
+    a.page_table = c.d_page_table;
+    a.pt_stride = c.pt_stride;
+    a.n_pages = (int)c.n_pages;
+    a.row_start = d_row_start;
+    a.past = d_past;
+    a.n_seqs = (int)n_seqs;
+    a.rows = (int)rows;
+    a.mask = tree ? d_mask : nullptr;
+    a.mask_words = (int)mask_words;
+    a.n_heads = (int)n_heads;
+    a.n_kv = (int)c.n_kv_heads;
+    a.head_dim = (int)hd;
+    a.scale = scale;
+    a.out = d_out;
+    a.ldo = ldo;
+    a.workspace = d_workspace;
+    a.err = nullptr; // the library's own word, reported by aaedn_device_sync
+    return attn_rows(a, as_stream(stream));
+}
+
+} // namespace
+
+extern "C" int aaedn_cu_attention_packed(const float* d_q, size_t ldq, const aaedn_kv_cache* cache,
+                                         const int32_t* d_row_start, const int32_t* d_past, size_t n_seqs, size_t rows,
+                                         size_t n_heads, float scale, float* d_out, size_t ldo, void* d_workspace,
+                                         size_t workspace_bytes, void* stream)
+{
+    return rows_call("aaedn_cu_attention_packed", false, d_q, ldq, cache, d_row_start, d_past, nullptr, 0, n_seqs, rows,
+                     n_heads, scale, d_out, ldo, d_workspace, workspace_bytes, stream);
+}
+
+extern "C" int aaedn_cu_attention_tree(const float* d_q, size_t ldq, const aaedn_kv_cache* cache,
+                                       const int32_t* d_row_start, const int32_t* d_past, const uint64_t* d_mask,
+                                       size_t mask_words, size_t n_seqs, size_t rows, size_t n_heads, float scale,
+                                       float* d_out, size_t ldo, void* d_workspace, size_t workspace_bytes, void* stream)
+{
+    return rows_call("aaedn_cu_attention_tree", true, d_q, ldq, cache, d_row_start, d_past, d_mask, mask_words, n_seqs,
+                     rows, n_heads, scale, d_out, ldo, d_workspace, workspace_bytes, stream);
+}

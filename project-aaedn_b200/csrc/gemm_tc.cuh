@@ -240,7 +240,8 @@ __device__ __forceinline__ void tc_pair_epilogue(const TcEpi& e, int m, int rbas
         if (isq || isk)
         {
             // rotate-half at the absolute position (D3, src/rope.cpp:53-54)
-            const float c = e.rope_cos[(size_t)pos * half + i], sn = e.rope_sin[(size_t)pos * half + i];
+            const int rp = e.row_rope ? e.row_rope[m] : pos;
+            const float c = e.rope_cos[(size_t)rp * half + i], sn = e.rope_sin[(size_t)rp * half + i];
             const float o0 = __fsub_rn(__fmul_rn(c, v), __fmul_rn(sn, u));
             const float o1 = __fadd_rn(__fmul_rn(sn, v), __fmul_rn(c, u));
             float* dst = isq ? e.qrows + (size_t)m * e.ldq + (size_t)h * hd : kv;

@@ -54,6 +54,7 @@ struct TcEpi
     const int* row_pos;
     const int* row_seq;
     int pt_stride;
+    const int* row_rope; // rope position of row m where it is not its slot (drafted trees); null: the slot
     const float* rope_cos; // [max_seq][head_dim / 2]
     const float* rope_sin;
     float* act; // [M][ld_act]

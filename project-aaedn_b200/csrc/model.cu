@@ -20,10 +20,13 @@
 #include <vector>
 
 #include "attention.cuh"
+#include "attn_rows.h"
 #include "gemm_tc.h"
 #include "gemv_q4.cuh"
 #include "gemv_tiled.cuh"
+#include "kv_pages.h"
 #include "prefill.cuh"
+#include "sample_rows.h"
 #include "tp.cuh"
 
 namespace aaedn_dev
@@ -443,6 +446,44 @@ int set_model_kernel_attrs()
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+// The index arrays of a chunk of packed rows, one block of memory (carved
+// alike on the host and the device, copied whole).
+constexpr int TREE_MAX_NODES = 256, TREE_MASK_WORDS = TREE_MAX_NODES / 64;
+struct RowsPlan
+{
+    uint8_t* base;
+    uint64_t* mask;                        // [rows][TREE_MASK_WORDS]
+    uint32_t* tokens;                      // [rows]
+    int *slot, *rope, *seq;                // [rows]: cache slot, rope position, sequence
+    int *row_start, *past, *seq_of, *last; // [seqs + 1], [seqs] x 3
+    float *temperature, *top_p, *min_p, *u; // [rows]
+    int* top_k;                             // [rows]
+    static size_t bytes(size_t rows, size_t seqs)
+    {
+        return rows * (TREE_MASK_WORDS * 8 + 9 * 4) + (4 * seqs + 1) * 4;
+    }
+    static RowsPlan carve(uint8_t* p, size_t rows, size_t seqs)
+    {
+        RowsPlan r{};
+        r.base = p;
+        auto next = [&p](size_t b) {
+            uint8_t* at = p;
+            p += b;
+            return at;
+        };
+        r.mask = reinterpret_cast<uint64_t*>(next(rows * TREE_MASK_WORDS * 8));
+        r.tokens = reinterpret_cast<uint32_t*>(next(rows * 4));
+        for (int** a : {&r.slot, &r.rope, &r.seq, &r.top_k})
+            *a = reinterpret_cast<int*>(next(rows * 4));
+        for (float** a : {&r.temperature, &r.top_p, &r.min_p, &r.u})
+            *a = reinterpret_cast<float*>(next(rows * 4));
+        r.row_start = reinterpret_cast<int*>(next((seqs + 1) * 4));
+        for (int** a : {&r.past, &r.seq_of, &r.last})
+            *a = reinterpret_cast<int*>(next(seqs * 4));
+        return r;
+    }
+};
+
 } // namespace
 
 struct aaedn_model
@@ -515,10 +556,18 @@ struct aaedn_model
         bool open = false;
         uint32_t len = 0;
         std::vector<int> pages;
+        std::vector<int> draft; // parents of the drafted nodes in slots len.. (step_tree, until accept)
     };
     std::vector<Seq> seqs;
     std::vector<int> page_ref, free_pages, h_pt;
     int* pinned_b = nullptr; // host staging: tokens, positions, sequences of a batch
+    // packed rows (prefill_batch, step_tree): the index arrays of one chunk,
+    // on the host (pinned) and the device, and the attention's workspace
+    RowsPlan h_plan{}, d_plan{};
+    void* attn_ws = nullptr;
+    std::vector<float*> kv_pools; // K and V of every layer
+    KvPairs cow{};                // page copies that reserve() has collected
+    int n_cow = 0;
 
     template <typename T>
     T* take(size_t bytes)
@@ -607,6 +656,14 @@ static size_t plan_arena(aaedn_model* m, bool carve)
         m->b_parts = std::max((int)((V + LR_BN - 1) / LR_BN), 2 * sm_count());
         m->b_pval = m->take<float>(S * (size_t)m->b_parts * 4);
         m->b_pidx = m->take<int>(S * (size_t)m->b_parts * 4);
+        m->d_plan = RowsPlan::carve(m->take<uint8_t>(RowsPlan::bytes((size_t)m->pf_rows, S)), (size_t)m->pf_rows, S);
+        m->attn_ws = m->take<uint8_t>(AAEDN_ATTN_ROWS_WORKSPACE_BYTES);
+        if (carve)
+            for (const DevLayer& L : m->layers)
+            {
+                m->kv_pools.push_back(L.k);
+                m->kv_pools.push_back(L.v);
+            }
     }
     return align_up(m->used, 256);
 }
@@ -1046,7 +1103,10 @@ static int put_tokens(aaedn_model* m, const uint32_t* h_tokens, size_t n)
 // Where the rows of a layer pass sit: row t at position pos0 + t of the one
 // sequence whose page table is page_table (a prefill chunk), or, with
 // row_pos / row_seq, at position row_pos[t] of sequence row_seq[t] whose page
-// table starts at page_table + row_seq[t] * pt_stride (batched decode).
+// table starts at page_table + row_seq[t] * pt_stride (batched decode). With
+// n_seqs, the rows are packed: several of each sequence, attended as
+// AttnRowsArgs says (row_start, past, seq_of; mask: drafted trees, whose rope
+// positions row_rope differ from their slots row_pos).
 struct RowMap
 {
     const int* page_table;
@@ -1054,6 +1114,9 @@ struct RowMap
     const int* row_pos;
     const int* row_seq;
     int pt_stride;
+    int n_seqs = 0;
+    const int *row_start = nullptr, *past = nullptr, *seq_of = nullptr, *row_rope = nullptr;
+    const uint64_t* mask = nullptr;
 };
 
 // The transformer layers over n residual rows in m->pf_hidden (the token
@@ -1101,11 +1164,40 @@ static int layers_pass(aaedn_model* m, int n, const RowMap& rm)
         q.e.row_pos = rm.row_pos;
         q.e.row_seq = rm.row_seq;
         q.e.pt_stride = rm.pt_stride;
+        q.e.row_rope = rm.row_rope;
         q.e.rope_cos = m->rope_cos;
         q.e.rope_sin = m->rope_sin;
         if ((rc = tc_gemm(q, st)))
             return rc;
-        if (rm.row_pos)
+        if (rm.n_seqs)
+        {
+            AttnRowsArgs a{};
+            a.q = m->pf_q;
+            a.ldq = (size_t)H * hd;
+            a.k = L.k;
+            a.v = L.v;
+            a.page_table = rm.page_table;
+            a.pt_stride = (size_t)rm.pt_stride;
+            a.seq_of = rm.seq_of;
+            a.n_pages = m->n_pages;
+            a.row_start = rm.row_start;
+            a.past = rm.past;
+            a.n_seqs = rm.n_seqs;
+            a.rows = n;
+            a.mask = rm.mask;
+            a.mask_words = TREE_MASK_WORDS;
+            a.n_heads = H;
+            a.n_kv = KV;
+            a.head_dim = hd;
+            a.scale = 1.0f / std::sqrt((float)hd); // src/transformer.cpp:198
+            a.out = m->pf_attn;
+            a.ldo = m->kpo;
+            a.workspace = m->attn_ws;
+            a.err = m->pf_err;
+            if ((rc = attn_rows(a, st)))
+                return rc;
+        }
+        else if (rm.row_pos)
         {
             // batched decode: one query row per sequence, the decode kernel
             // with a cluster of S splits per (kv head, row), S making about
@@ -1397,6 +1489,10 @@ static int create_impl(const aaedn_model_config* cfg, uint32_t tp_rank, uint32_t
     {
         if (cudaMallocHost(reinterpret_cast<void**>(&m->pinned_b), (size_t)m->max_seqs * 3 * 4) != cudaSuccess)
             return fail(set_error(AAEDN_ENOMEM, "pinned staging allocation failed"));
+        uint8_t* hp = nullptr;
+        if (cudaMallocHost(reinterpret_cast<void**>(&hp), RowsPlan::bytes((size_t)m->pf_rows, m->max_seqs)) != cudaSuccess)
+            return fail(set_error(AAEDN_ENOMEM, "pinned staging allocation failed"));
+        m->h_plan = RowsPlan::carve(hp, (size_t)m->pf_rows, m->max_seqs);
         m->seqs.assign(m->max_seqs, aaedn_model::Seq{});
         m->page_ref.assign((size_t)m->n_pages, 0);
         m->free_pages.resize((size_t)m->n_pages);
@@ -1457,6 +1553,8 @@ static int create_impl(const aaedn_model_config* cfg, uint32_t tp_rank, uint32_t
             m->attn_warps = nw;
     }
     rc = set_model_kernel_attrs();
+    if (!rc)
+        rc = attn_rows_init();
     if (rc)
         return fail(rc);
     if (m->tp_size > 1)
@@ -1563,6 +1661,8 @@ extern "C" int aaedn_model_destroy(aaedn_model* m)
         cudaFreeHost(m->pinned);
     if (m->pinned_b)
         cudaFreeHost(m->pinned_b);
+    if (m->h_plan.base)
+        cudaFreeHost(m->h_plan.base);
     if (m->stream)
         cudaStreamDestroy(m->stream);
     delete m;
@@ -2259,13 +2359,43 @@ static void release_pages(aaedn_model* m, std::vector<int>& pages)
     pages.clear();
 }
 
+// Gives back the pages behind sequence seq's last token (what a draft that
+// was not accepted, or a call that failed, left reserved).
+static int trim(aaedn_model* m, uint32_t seq)
+{
+    auto& sq = m->seqs[seq];
+    sq.draft.clear();
+    const size_t need = ((size_t)sq.len + m->page_size - 1) / m->page_size;
+    if (sq.pages.size() <= need)
+        return AAEDN_OK;
+    std::vector<int> rest(sq.pages.begin() + (ptrdiff_t)need, sq.pages.end());
+    sq.pages.resize(need);
+    release_pages(m, rest);
+    return upload_pt(m, seq);
+}
+
+// Enqueues the page copies that reserve() collected: one launch for every
+// layer's K and V.
+static int flush_copies(aaedn_model* m)
+{
+    const int n = m->n_cow;
+    m->n_cow = 0;
+    if (n == 0)
+        return AAEDN_OK;
+    return kv_copy_pages_host(m->kv_pools.data(), m->kv_pools.size(),
+                              (size_t)m->cfg.n_kv_heads * m->page_size * m->cfg.head_dim, m->n_pages, m->cow, n,
+                              m->stream);
+}
+
 // Pages for positions [len, len + n) of sequence seq: new pages from the
 // pool, and a copy of the page holding position len when another sequence
-// shares it (its rows below len stay valid in both).
+// shares it (its rows below len stay valid in both). A draft that was not
+// accepted is dropped. The copies are enqueued by flush_copies.
 static int reserve(aaedn_model* m, uint32_t seq, uint32_t n)
 {
     auto& sq = m->seqs[seq];
     const uint32_t P = (uint32_t)m->page_size;
+    sq.draft.clear();
     if ((size_t)sq.len + n > m->cfg.max_seq)
         return set_error(AAEDN_ESTATE, "sequence %u full: %u + %u tokens > max_seq %u", seq, sq.len, n, m->cfg.max_seq);
     bool changed = false;
@@ -2279,14 +2409,11 @@ static int reserve(aaedn_model* m, uint32_t seq, uint32_t n)
                 return set_error(AAEDN_ENOMEM, "KV page pool exhausted (%d pages)", m->n_pages);
             const int fresh = m->free_pages.back();
             m->free_pages.pop_back();
-            const size_t pe = (size_t)m->cfg.n_kv_heads * P * m->cfg.head_dim; // floats per page per layer
-            for (const DevLayer& L : m->layers)
-            {
-                AAEDN_CUDA_TRY(cudaMemcpyAsync(L.k + (size_t)fresh * pe, L.k + (size_t)old * pe, pe * 4,
-                                               cudaMemcpyDeviceToDevice, m->stream));
-                AAEDN_CUDA_TRY(cudaMemcpyAsync(L.v + (size_t)fresh * pe, L.v + (size_t)old * pe, pe * 4,
-                                               cudaMemcpyDeviceToDevice, m->stream));
-            }
+            // a fresh page is nobody's source and a source stays held by its
+            // other sequences, so the collected copies do not depend on one another
+            m->cow.src[m->n_cow] = old;
+            m->cow.dst[m->n_cow] = fresh;
+            ++m->n_cow;
             --m->page_ref[(size_t)old];
             m->page_ref[(size_t)fresh] = 1;
             sq.pages[pi] = fresh;
@@ -2294,28 +2421,62 @@ static int reserve(aaedn_model* m, uint32_t seq, uint32_t n)
         }
     }
     const size_t need = ((size_t)sq.len + n + P - 1) / P;
-    while (sq.pages.size() < need)
+    int rc = AAEDN_OK;
+    while (!rc && sq.pages.size() < need)
     {
         if (m->free_pages.empty())
-            return set_error(AAEDN_ENOMEM, "KV page pool exhausted (%d pages)", m->n_pages);
+        {
+            rc = set_error(AAEDN_ENOMEM, "KV page pool exhausted (%d pages)", m->n_pages);
+            break;
+        }
         const int pg = m->free_pages.back();
         m->free_pages.pop_back();
         m->page_ref[(size_t)pg] = 1;
         sq.pages.push_back(pg);
         changed = true;
     }
-    return changed ? upload_pt(m, seq) : AAEDN_OK;
+    if (m->n_cow == KV_MAX_PAIRS || rc) // full, or the caller gives up: the pages that moved are copied all the same
+        if (int crc = flush_copies(m))
+            return crc;
+    if (changed)
+        if (int urc = upload_pt(m, seq))
+            return urc;
+    return rc;
+}
+
+// reserve() for several sequences; on a failure the pages of the earlier
+// ones are given back.
+static int reserve_all(aaedn_model* m, const uint32_t* seqs, const uint32_t* counts, size_t n)
+{
+    for (size_t i = 0; i < n; ++i)
+        if (int rc = reserve(m, seqs[i], counts ? counts[i] : 1u))
+        {
+            for (size_t j = 0; j <= i; ++j)
+                trim(m, seqs[j]);
+            flush_copies(m);
+            return rc;
+        }
+    return flush_copies(m);
 }
 
 // The final RMSNorm, lm_head and greedy token of n rows of m->pf_hidden
 // starting at row0, into b_logits / b_next rows [0, n).
-static int lm_rows(aaedn_model* m, int row0, int n)
+// (with d_rows: rows d_rows[0..n) of it instead).
+static int lm_rows(aaedn_model* m, int row0, int n, const int* d_rows = nullptr)
 {
     cudaStream_t st = m->stream;
     const int D = (int)m->cfg.dim, V = (int)m->cfg.vocab;
-    pf_rmsnorm_rows_kernel<<<n, 256, 0, st>>>(m->pf_hidden + (size_t)row0 * D, D, m->final_norm, m->cfg.eps,
-                                               m->b_norm);
-    AAEDN_LAUNCH_CHECK("pf_rmsnorm_rows_kernel");
+    if (d_rows)
+    {
+        pf_rmsnorm_gather_kernel<<<n, 256, 0, st>>>(m->pf_hidden, d_rows, D, m->final_norm, m->cfg.eps, m->b_norm);
+        AAEDN_LAUNCH_CHECK("pf_rmsnorm_gather_kernel");
+    }
+    else
+    {
+        pf_rmsnorm_rows_kernel<<<n, 256, 0, st>>>(m->pf_hidden + (size_t)row0 * D, D, m->final_norm, m->cfg.eps,
+                                                   m->b_norm);
+        AAEDN_LAUNCH_CHECK("pf_rmsnorm_rows_kernel");
+    }
     int parts;
     if (n <= LF_MAXM && D % 128 == 0)
     {
@@ -2372,6 +2533,12 @@ extern "C" int aaedn_seq_fork(aaedn_model* m, uint32_t parent, uint32_t* child)
     uint32_t c = 0;
     if (int rc = aaedn_seq_open(m, &c))
         return rc;
+    // the child shares the pages of the parent's tokens only
+    if (int rc = trim(m, parent))
+    {
+        m->seqs[c].open = false;
+        return rc;
+    }
     m->seqs[c].len = m->seqs[parent].len;
     m->seqs[c].pages = m->seqs[parent].pages;
     for (int pg : m->seqs[c].pages)
@@ -2392,6 +2559,7 @@ extern "C" int aaedn_seq_close(aaedn_model* m, uint32_t seq)
     release_pages(m, m->seqs[seq].pages);
     m->seqs[seq].open = false;
     m->seqs[seq].len = 0;
+    m->seqs[seq].draft.clear();
     return AAEDN_OK;
 }
 
@@ -2427,7 +2595,10 @@ extern "C" int aaedn_seq_prefill(aaedn_model* m, uint32_t seq, const uint32_t* h
     for (size_t i = 0; i < n; ++i)
         if (h_tokens[i] >= m->cfg.vocab)
             return set_error(AAEDN_EINVAL, "token id %u >= vocab %u", h_tokens[i], m->cfg.vocab);
-    if (int rc = reserve(m, seq, (uint32_t)n))
+    if (n > m->cfg.max_seq)
+        return set_error(AAEDN_ESTATE, "sequence %u full: %zu tokens > max_seq %u", seq, n, m->cfg.max_seq);
+    const uint32_t n32 = (uint32_t)n;
+    if (int rc = reserve_all(m, &seq, &n32, 1))
         return rc;
     // tokens into the model's prompt buffer (the staging is reused only
     // after the stream has drained)
@@ -2456,25 +2627,90 @@ extern "C" int aaedn_seq_prefill(aaedn_model* m, uint32_t seq, const uint32_t* h
     return device_status(m);
 }
 
-extern "C" int aaedn_model_step_batch(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_tokens, size_t n,
-                                      float* h_logits, uint32_t* h_next)
+// The tokens that follow rows [0, n) of b_logits: sampled with rows
+// [first, first + n) of the plan's parameters (already on the device), or the
+// greedy ones of lm_rows.
+static int draw_rows(aaedn_model* m, const aaedn_sampling* sp, size_t first, size_t n)
 {
-    BATCHED_OK(m);
+    if (!sp)
+        return AAEDN_OK;
+    SampleRowsArgs a{};
+    a.logits = m->b_logits;
+    a.ld = m->cfg.vocab;
+    a.rows = (uint32_t)n;
+    a.vocab = m->cfg.vocab;
+    a.temperature = sp->h_temperature ? m->d_plan.temperature + first : nullptr;
+    a.top_k = sp->h_top_k ? m->d_plan.top_k + first : nullptr;
+    a.top_p = sp->h_top_p ? m->d_plan.top_p + first : nullptr;
+    a.min_p = sp->h_min_p ? m->d_plan.min_p + first : nullptr;
+    a.u = m->d_plan.u + first;
+    a.tokens = m->b_next;
+    return sample_rows(a, m->stream);
+}
+
+// Rows [0, n) of the plan's sampling parameters = rows first.. of sp.
+static void put_sampling(aaedn_model* m, const aaedn_sampling* sp, size_t first, size_t n)
+{
+    if (!sp)
+        return;
+    const RowsPlan& h = m->h_plan;
+    if (sp->h_temperature)
+        std::memcpy(h.temperature, sp->h_temperature + first, n * 4);
+    if (sp->h_top_k)
+        std::memcpy(h.top_k, sp->h_top_k + first, n * 4);
+    if (sp->h_top_p)
+        std::memcpy(h.top_p, sp->h_top_p + first, n * 4);
+    if (sp->h_min_p)
+        std::memcpy(h.min_p, sp->h_min_p + first, n * 4);
+    std::memcpy(h.u, sp->h_u + first, n * 4);
+}
+
+static int sampling_ok(aaedn_model* m, const char* fn, const aaedn_sampling* sp)
+{
+    if (sp && !sp->h_u)
+        return set_error(AAEDN_EINVAL, "%s: sampling without uniforms (h_u)", fn);
+    if (sp && m->cfg.vocab > SR_MAX_VOCAB)
+        return set_error(AAEDN_EUNSUPPORTED, "%s: sampling takes a vocabulary of at most %u", fn, SR_MAX_VOCAB);
+    return AAEDN_OK;
+}
+
+static int push_plan(aaedn_model* m)
+{
+    AAEDN_CUDA_TRY(cudaMemcpyAsync(m->d_plan.base, m->h_plan.base, RowsPlan::bytes((size_t)m->pf_rows, m->max_seqs),
+                                   cudaMemcpyHostToDevice, m->stream));
+    return AAEDN_OK;
+}
+
+// Open, listed once, and the tokens in the vocabulary.
+static int batch_ok(aaedn_model* m, const char* fn, const uint32_t* h_seqs, const uint32_t* h_counts,
+                    const uint32_t* h_tokens, size_t n, size_t* total)
+{
     if (!h_seqs || !h_tokens || n == 0 || n > m->max_seqs)
-        return set_error(AAEDN_EINVAL, "aaedn_model_step_batch: 1..%u sequences", m->max_seqs);
+        return set_error(AAEDN_EINVAL, "%s: 1..%u sequences", fn, m->max_seqs);
     std::vector<uint8_t> seen(m->max_seqs, 0);
+    size_t sum = 0;
     for (size_t i = 0; i < n; ++i)
     {
         if (int rc = seq_ok(m, h_seqs[i]))
             return rc;
         if (seen[h_seqs[i]]++)
             return set_error(AAEDN_EINVAL, "sequence %u twice in one batch", h_seqs[i]);
+        if (h_counts && h_counts[i] == 0)
+            return set_error(AAEDN_EINVAL, "%s: no tokens for sequence %u", fn, h_seqs[i]);
+        sum += h_counts ? h_counts[i] : 1u;
+    }
+    for (size_t i = 0; i < sum; ++i)
         if (h_tokens[i] >= m->cfg.vocab)
             return set_error(AAEDN_EINVAL, "token id %u >= vocab %u", h_tokens[i], m->cfg.vocab);
-    }
-    for (size_t i = 0; i < n; ++i)
-        if (int rc = reserve(m, h_seqs[i], 1))
-            return rc;
+    *total = sum;
+    return AAEDN_OK;
+}
+
+static int step_rows(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_tokens, size_t n,
+                     const aaedn_sampling* sp, float* h_logits, uint32_t* h_next)
+{
+    if (int rc = reserve_all(m, h_seqs, nullptr, n))
+        return rc;
     AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream)); // the staging may still feed an earlier copy
     int* stg = m->pinned_b;
     for (size_t i = 0; i < n; ++i)
@@ -2486,9 +2722,18 @@ extern "C" int aaedn_model_step_batch(aaedn_model* m, const uint32_t* h_seqs, co
     AAEDN_CUDA_TRY(cudaMemcpyAsync(m->b_tokens, stg, n * 4, cudaMemcpyHostToDevice, m->stream));
     AAEDN_CUDA_TRY(cudaMemcpyAsync(m->b_pos, stg + m->max_seqs, n * 4, cudaMemcpyHostToDevice, m->stream));
     AAEDN_CUDA_TRY(cudaMemcpyAsync(m->b_seq, stg + 2 * m->max_seqs, n * 4, cudaMemcpyHostToDevice, m->stream));
-    int rc = prefill_chunk(m, m->b_tokens, (int)n, RowMap{m->seq_pt, 0u, m->b_pos, m->b_seq, (int)m->pt_stride});
+    int rc = AAEDN_OK;
+    if (sp)
+    {
+        put_sampling(m, sp, 0, n);
+        rc = push_plan(m);
+    }
+    if (!rc)
+        rc = prefill_chunk(m, m->b_tokens, (int)n, RowMap{m->seq_pt, 0u, m->b_pos, m->b_seq, (int)m->pt_stride});
     if (!rc)
         rc = lm_rows(m, 0, (int)n);
+    if (!rc)
+        rc = draw_rows(m, sp, 0, n);
     if (rc)
         return rc;
     if (h_logits)
@@ -2500,4 +2745,262 @@ extern "C" int aaedn_model_step_batch(aaedn_model* m, const uint32_t* h_seqs, co
     for (size_t i = 0; i < n; ++i)
         ++m->seqs[h_seqs[i]].len;
     return device_status(m);
+}
+
+extern "C" int aaedn_model_step_batch(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_tokens, size_t n,
+                                      float* h_logits, uint32_t* h_next)
+{
+    BATCHED_OK(m);
+    size_t total = 0;
+    if (int rc = batch_ok(m, "aaedn_model_step_batch", h_seqs, nullptr, h_tokens, n, &total))
+        return rc;
+    return step_rows(m, h_seqs, h_tokens, n, nullptr, h_logits, h_next);
+}
+
+extern "C" int aaedn_model_step_sample(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_tokens, size_t n,
+                                       const aaedn_sampling* sampling, float* h_logits, uint32_t* h_next)
+{
+    BATCHED_OK(m);
+    const char* fn = "aaedn_model_step_sample";
+    size_t total = 0;
+    int rc;
+    if ((rc = batch_ok(m, fn, h_seqs, nullptr, h_tokens, n, &total)) || (rc = sampling_ok(m, fn, sampling)))
+        return rc;
+    return step_rows(m, h_seqs, h_tokens, n, sampling, h_logits, h_next);
+}
+
+extern "C" int aaedn_seq_prefill_batch(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts,
+                                       const uint32_t* h_tokens, size_t n, const aaedn_sampling* sampling,
+                                       float* h_logits, uint32_t* h_next)
+{
+    BATCHED_OK(m);
+    const char* fn = "aaedn_seq_prefill_batch";
+    if (!h_counts)
+        return set_error(AAEDN_EINVAL, "%s: null counts", fn);
+    size_t total = 0;
+    int rc;
+    if ((rc = batch_ok(m, fn, h_seqs, h_counts, h_tokens, n, &total)) || (rc = sampling_ok(m, fn, sampling)))
+        return rc;
+    if ((rc = reserve_all(m, h_seqs, h_counts, n)))
+        return rc;
+    const RowsPlan &h = m->h_plan, &d = m->d_plan;
+    const size_t V = m->cfg.vocab;
+    // the packed rows in chunks of pf_rows: a sequence may go on in the next
+    size_t i0 = 0, off0 = 0, tok0 = 0; // the chunk's first sequence, its tokens done, its first token
+    while (i0 < n)
+    {
+        AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream)); // the staging may still feed an earlier copy
+        size_t i = i0, off = off0, rows = 0, ns = 0, done = 0;
+        while (i < n && rows < (size_t)m->pf_rows)
+        {
+            const size_t take = std::min((size_t)h_counts[i] - off, (size_t)m->pf_rows - rows);
+            const int past = (int)(m->seqs[h_seqs[i]].len + off);
+            h.row_start[ns] = (int)rows;
+            h.past[ns] = past;
+            h.seq_of[ns] = (int)h_seqs[i];
+            for (size_t r = 0; r < take; ++r)
+            {
+                h.tokens[rows + r] = h_tokens[tok0 + rows + r];
+                h.slot[rows + r] = past + (int)r;
+                h.seq[rows + r] = (int)h_seqs[i];
+            }
+            rows += take;
+            ++ns;
+            off += take;
+            if (off == h_counts[i])
+            {
+                h.last[done++] = (int)rows - 1; // the sequence's last token
+                off = 0;
+                ++i;
+            }
+        }
+        h.row_start[ns] = (int)rows;
+        put_sampling(m, sampling, i0, done); // the chunk finishes sequences i0 .. i0 + done - 1
+        if ((rc = push_plan(m)))
+            return rc;
+        RowMap rm{m->seq_pt, 0u, d.slot, d.seq, (int)m->pt_stride};
+        rm.n_seqs = (int)ns;
+        rm.row_start = d.row_start;
+        rm.past = d.past;
+        rm.seq_of = d.seq_of;
+        if ((rc = prefill_chunk(m, d.tokens, (int)rows, rm)))
+            return rc;
+        if (done)
+        {
+            if ((rc = lm_rows(m, 0, (int)done, d.last)) || (rc = draw_rows(m, sampling, 0, done)))
+                return rc;
+            if (h_logits)
+                AAEDN_CUDA_TRY(cudaMemcpyAsync(h_logits + i0 * V, m->b_logits, done * V * 4, cudaMemcpyDeviceToHost,
+                                               m->stream));
+            if (h_next)
+                AAEDN_CUDA_TRY(cudaMemcpyAsync(h_next + i0, m->b_next, done * 4, cudaMemcpyDeviceToHost, m->stream));
+        }
+        i0 = i;
+        off0 = off;
+        tok0 += rows;
+    }
+    AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream));
+    for (size_t i = 0; i < n; ++i)
+        m->seqs[h_seqs[i]].len += h_counts[i];
+    return device_status(m);
+}
+
+extern "C" int aaedn_model_step_tree(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts,
+                                     const uint32_t* h_tokens, const int32_t* h_parents, size_t n,
+                                     const aaedn_sampling* sampling, float* h_logits, uint32_t* h_next)
+{
+    BATCHED_OK(m);
+    const char* fn = "aaedn_model_step_tree";
+    if (!h_counts || !h_parents)
+        return set_error(AAEDN_EINVAL, "%s: null counts or parents", fn);
+    size_t total = 0;
+    int rc;
+    if ((rc = batch_ok(m, fn, h_seqs, h_counts, h_tokens, n, &total)) || (rc = sampling_ok(m, fn, sampling)))
+        return rc;
+    if (total > (size_t)m->pf_rows)
+        return set_error(AAEDN_EINVAL, "%s: %zu nodes, at most %d in one step", fn, total, m->pf_rows);
+    for (size_t i = 0, t = 0; i < n; t += h_counts[i], ++i)
+    {
+        if (h_counts[i] > (uint32_t)TREE_MAX_NODES)
+            return set_error(AAEDN_EINVAL, "%s: %u nodes of sequence %u, at most %d", fn, h_counts[i], h_seqs[i],
+                             TREE_MAX_NODES);
+        for (uint32_t j = 0; j < h_counts[i]; ++j)
+            if (h_parents[t + j] < -1 || h_parents[t + j] >= (int32_t)j)
+                return set_error(AAEDN_EINVAL, "%s: the parent %d of node %u is not -1 or an earlier node", fn,
+                                 h_parents[t + j], j);
+    }
+    if ((rc = reserve_all(m, h_seqs, h_counts, n)))
+        return rc;
+    AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream)); // the staging may still feed an earlier copy
+    const RowsPlan &h = m->h_plan, &d = m->d_plan;
+    std::memset(h.mask, 0, total * TREE_MASK_WORDS * 8);
+    size_t t = 0;
+    for (size_t i = 0; i < n; ++i)
+    {
+        const int len = (int)m->seqs[h_seqs[i]].len;
+        h.row_start[i] = (int)t;
+        h.past[i] = len;
+        h.seq_of[i] = (int)h_seqs[i];
+        for (uint32_t j = 0; j < h_counts[i]; ++j)
+        {
+            const int par = h_parents[t + j];
+            uint64_t* w = h.mask + (t + j) * TREE_MASK_WORDS;
+            if (par >= 0)
+                std::memcpy(w, h.mask + (t + (size_t)par) * TREE_MASK_WORDS, TREE_MASK_WORDS * 8);
+            w[j >> 6] |= 1ull << (j & 63);
+            h.tokens[t + j] = h_tokens[t + j];
+            h.slot[t + j] = len + (int)j;
+            h.rope[t + j] = par < 0 ? len : h.rope[t + (size_t)par] + 1; // its depth behind the sequence
+            h.seq[t + j] = (int)h_seqs[i];
+        }
+        t += h_counts[i];
+    }
+    h.row_start[n] = (int)t;
+    put_sampling(m, sampling, 0, total);
+    if ((rc = push_plan(m)))
+        return rc;
+    RowMap rm{m->seq_pt, 0u, d.slot, d.seq, (int)m->pt_stride};
+    rm.n_seqs = (int)n;
+    rm.row_start = d.row_start;
+    rm.past = d.past;
+    rm.seq_of = d.seq_of;
+    rm.row_rope = d.rope;
+    rm.mask = d.mask;
+    if ((rc = prefill_chunk(m, d.tokens, (int)total, rm)))
+        return rc;
+    const size_t V = m->cfg.vocab;
+    for (size_t r0 = 0; r0 < total; r0 += m->max_seqs) // the logits buffer holds max_seqs rows
+    {
+        const size_t nr = std::min<size_t>(m->max_seqs, total - r0);
+        if ((rc = lm_rows(m, (int)r0, (int)nr)) || (rc = draw_rows(m, sampling, r0, nr)))
+            return rc;
+        if (h_logits)
+            AAEDN_CUDA_TRY(cudaMemcpyAsync(h_logits + r0 * V, m->b_logits, nr * V * 4, cudaMemcpyDeviceToHost,
+                                           m->stream));
+        if (h_next)
+            AAEDN_CUDA_TRY(cudaMemcpyAsync(h_next + r0, m->b_next, nr * 4, cudaMemcpyDeviceToHost, m->stream));
+    }
+    AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream));
+    t = 0;
+    for (size_t i = 0; i < n; ++i)
+    {
+        m->seqs[h_seqs[i]].draft.assign(h_parents + t, h_parents + t + h_counts[i]);
+        t += h_counts[i];
+    }
+    return device_status(m);
+}
+
+extern "C" int aaedn_seq_accept(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts,
+                                const uint32_t* h_nodes, size_t n)
+{
+    BATCHED_OK(m);
+    const char* fn = "aaedn_seq_accept";
+    if (!h_seqs || !h_counts || n == 0 || n > m->max_seqs)
+        return set_error(AAEDN_EINVAL, "%s: 1..%u sequences", fn, m->max_seqs);
+    std::vector<uint8_t> seen(m->max_seqs, 0);
+    size_t total = 0;
+    for (size_t i = 0; i < n; ++i)
+    {
+        if (int rc = seq_ok(m, h_seqs[i]))
+            return rc;
+        if (seen[h_seqs[i]]++)
+            return set_error(AAEDN_EINVAL, "sequence %u twice in one batch", h_seqs[i]);
+        const auto& draft = m->seqs[h_seqs[i]].draft;
+        if (draft.empty())
+            return set_error(AAEDN_ESTATE, "%s: sequence %u has no drafted tree", fn, h_seqs[i]);
+        if (h_counts[i] && !h_nodes)
+            return set_error(AAEDN_EINVAL, "%s: null nodes", fn);
+        int32_t prev = -1;
+        for (uint32_t j = 0; j < h_counts[i]; ++j)
+        {
+            const uint32_t node = h_nodes[total + j];
+            if (node >= draft.size() || draft[node] != prev)
+                return set_error(AAEDN_EINVAL, "%s: node %u of sequence %u does not follow node %d", fn, node, h_seqs[i],
+                                 prev);
+            prev = (int32_t)node;
+        }
+        total += h_counts[i];
+    }
+    AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream)); // the staging may still feed an earlier copy
+    const RowsPlan &h = m->h_plan, &d = m->d_plan;
+    size_t t = 0;
+    bool moves = false;
+    for (size_t i = 0; i < n; ++i)
+    {
+        h.row_start[i] = (int)t;
+        h.past[i] = (int)m->seqs[h_seqs[i]].len;
+        h.seq_of[i] = (int)h_seqs[i];
+        for (uint32_t j = 0; j < h_counts[i]; ++j, ++t) // a path's nodes ascend: parents are earlier nodes
+        {
+            h.slot[t] = (int)h_nodes[t];
+            moves |= h_nodes[t] != j;
+        }
+    }
+    h.row_start[n] = (int)t;
+    if (moves)
+    {
+        if (int rc = push_plan(m))
+            return rc;
+        KvCompactArgs a{};
+        a.n_pages = m->n_pages;
+        a.n_kv = (int)m->cfg.n_kv_heads;
+        a.head_dim = (int)m->cfg.head_dim;
+        a.page_table = m->seq_pt;
+        a.pt_stride = m->pt_stride;
+        a.seq_of = d.seq_of;
+        a.base = d.past;
+        a.keep = d.slot;
+        a.keep_start = d.row_start;
+        a.n_seqs = (int)n;
+        a.n_keep = (int)t;
+        if (int rc = kv_compact(m->kv_pools.data(), m->kv_pools.size(), a, m->stream))
+            return rc;
+    }
+    for (size_t i = 0; i < n; ++i)
+    {
+        m->seqs[h_seqs[i]].len += h_counts[i];
+        if (int rc = trim(m, h_seqs[i]))
+            return rc;
+    }
+    return AAEDN_OK;
 }

@@ -343,6 +343,23 @@ __global__ void __launch_bounds__(256) pf_rmsnorm_rows_kernel(const float* __res
         out[(size_t)blockIdx.x * D + k] = __fmul_rn(__fmul_rn(xr[k], rms), gain[k]);
 }
 
+// The same for the rows rows[m] of x (a batch's last tokens).
+__global__ void __launch_bounds__(256) pf_rmsnorm_gather_kernel(const float* __restrict__ x,
+                                                                const int* __restrict__ rows, int D,
+                                                                const float* __restrict__ gain, float eps,
+                                                                float* __restrict__ out)
+{
+    __shared__ float scratch[64];
+    const float* xr = x + (size_t)rows[blockIdx.x] * D;
+    float ss = 0.0f;
+    for (int k = threadIdx.x; k < D; k += blockDim.x)
+        ss = fmaf(xr[k], xr[k], ss);
+    ss = block_sum(ss, scratch);
+    const float rms = 1.0f / sqrtf(__fadd_rn(__fdiv_rn(ss, (float)D), eps));
+    for (int k = threadIdx.x; k < D; k += blockDim.x)
+        out[(size_t)blockIdx.x * D + k] = __fmul_rn(__fmul_rn(xr[k], rms), gain[k]);
+}
+
 // Greedy-token partials: a CTA's best (value, id) per activation row over its
 // vocabulary rows, ties to the lowest id; argmax_parts_kernel takes the best
 // of a row's partials in order.

@@ -1,0 +1,611 @@
+// sample_rows.cu — next tokens of many rows of logits in one launch:
+// temperature, top-k, min-p, top-p and a multinomial draw per row from the
+// caller's uniforms, the many-row form of sample.cu with its order of the
+// vocabulary (logit descending, ties by the lower id).
+//
+// With M the row's largest logit and p_i = exp((l_i - M) / T), the kept
+// tokens are a prefix of that order: the first top_k of them; of those the
+// ones with p_i >= min_p; of those, up to and including the first whose
+// cumulative mass reaches top_p times their mass. The token is the first
+// kept one whose cumulative mass reaches u times the kept mass. So every
+// step is one search: the first token in the order whose cumulative count
+// (top_k) or cumulative mass (top_p, the draw) reaches a target; min_p only
+// takes masses out of the sums.
+//
+// p is computed in fp64 (2^-52 relative; B200 runs fp64 at half the fp32
+// rate) and held as an integer number of units of 2^-45: sums of integers
+// are exact in any order, so the result does not depend on the order of the
+// atomics. The units' rounding moves a cumulative sum by at most 2^-46 a
+// token, below 2^-29 of the mass for a million tokens, and a uniform has 24
+// bits.
+//
+// A row is a thread-block cluster of C CTAs, each with a slice of the
+// vocabulary in registers (one read of the logits). One pass makes a
+// histogram (count and mass) over 1024 equal steps of M - l; a search picks
+// the step that crosses its target, gathers that step's few tokens in the
+// first CTA, sorts them and scans their masses. A step with more tokens
+// than the list holds (ties, far outliers) is first narrowed by a radix
+// descent over (logit bits, id), 10 bits a pass.
+#include "common.cuh"
+
+#include "device_check.hpp"
+#include "sample_rows.h"
+
+namespace aaedn_dev
+{
+
+namespace
+{
+
+constexpr int SR_THREADS = 1024, SR_WARPS = SR_THREADS / 32;
+constexpr int SR_BINS = 1024; // one per thread
+constexpr int SR_LIST = 512;
+constexpr int SR_MASS_BITS = 45;
+
+struct SrShared
+{
+    uint32_t cnt[SR_BINS], m0[SR_BINS], m1[SR_BINS], m2[SR_BINS]; // this CTA's histogram
+    uint64_t pm[SR_BINS];                                         // cumulative mass of the row's steps
+    uint32_t pc[SR_BINS];                                         // cumulative count
+    uint64_t lkey[SR_LIST], lmass[SR_LIST], skey[SR_LIST], smass[SR_LIST];
+    double tbl[64]; // 2^(j / 64)
+    uint64_t wsum_m[SR_WARPS];
+    uint32_t wsum_c[SR_WARPS];
+    float red_max[SR_WARPS], red_min[SR_WARPS];
+    uint32_t red_idx[SR_WARPS];
+    float cta_max, cta_min;
+    uint32_t cta_idx;
+    uint32_t n_list;
+    int pick;
+    uint64_t above_m, tot_m;
+    uint32_t above_c, n_in;
+    uint64_t found_key, found_mass;
+};
+
+// ---- shared memory of the cluster's CTAs ------------------------------------
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank)
+{
+    uint32_t ra;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_addr(p)), "r"(rank));
+    return ra;
+}
+__device__ __forceinline__ uint32_t peer_ld32(uint32_t a)
+{
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void peer_st64(uint32_t a, uint64_t v)
+{
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t peer_add32(uint32_t a, uint32_t v)
+{
+    uint32_t r;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
+    return r;
+}
+
+template <int C>
+__device__ __forceinline__ void row_sync()
+{
+    if constexpr (C > 1)
+        cluster_sync_all();
+    else
+        __syncthreads();
+}
+
+// Larger = earlier in the order: the logit's bits as an ordered integer, then
+// the lower id.
+__device__ __forceinline__ uint64_t order_key(float l, uint32_t id)
+{
+    const uint32_t b = __float_as_uint(l == 0.0f ? 0.0f : l); // -0 ties with 0
+    const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    return ((uint64_t)o << 32) | (0xFFFFFFFFu - id);
+}
+
+// exp(x) for -33 <= x <= 0 by table lookup (P. T. P. Tang, "Table-driven
+// implementation of the exponential function in IEEE floating-point
+// arithmetic", 1989): x = k ln2 / 64 + r, exp(x) = 2^(k / 64) exp(r), the
+// polynomial of exp(r) to r^5 (|r| <= ln2 / 128: the next term is 4e-17).
+__device__ __forceinline__ double sr_exp(double x, const double* tbl)
+{
+    constexpr double LN2 = 0.69314718055994530942, MAGIC = 6755399441055744.0; // 1.5 * 2^52
+    const double t = fma(x, 64.0 / LN2, MAGIC);
+    const int k = __double2loint(t);
+    const double r = fma(t - MAGIC, -LN2 / 64.0, x);
+    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const double y = tbl[k & 63] * p;
+    return __hiloint2double(__double2hiint(y) + (k >> 6) * (1 << 20), __double2loint(y));
+}
+
+struct SrRow
+{
+    float M, invw;
+    double dM, inv_t, min_p;
+    float far; // M - l beyond which the mass rounds to zero units
+};
+
+__device__ __forceinline__ int sr_bin(float l, const SrRow& r)
+{
+    return min((int)((r.M - l) * r.invw), SR_BINS - 1); // monotone in l; NaN (0 * inf) counts as 0
+}
+
+// mass in units of 2^-45; 0 for tokens below min_p
+__device__ __forceinline__ uint64_t sr_mass(float l, const SrRow& r, const double* tbl)
+{
+    if (!(r.M - l <= r.far))
+        return 0;
+    const double y = sr_exp(fmax(((double)l - r.dM) * r.inv_t, -33.0), tbl);
+    if (y < r.min_p)
+        return 0;
+    constexpr double TWO52 = 4503599627370496.0;
+    return (uint64_t)__double_as_longlong(fma(y, (double)(1ull << SR_MASS_BITS), TWO52)) & ((1ull << 52) - 1);
+}
+
+// Inclusive scan over the CTA's threads of a count and a mass.
+__device__ __forceinline__ void sr_scan(uint32_t& c, uint64_t& m, SrShared& s)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const uint32_t oc = __shfl_up_sync(0xffffffffu, c, o);
+        const uint64_t om = __shfl_up_sync(0xffffffffu, m, o);
+        if (lane >= o)
+        {
+            c += oc;
+            m += om;
+        }
+    }
+    __syncthreads(); // the sums of the scan before are read
+    if (lane == 31)
+    {
+        s.wsum_c[warp] = c;
+        s.wsum_m[warp] = m;
+    }
+    __syncthreads();
+    uint32_t bc = lane < warp ? s.wsum_c[lane] : 0;
+    uint64_t bm = lane < warp ? s.wsum_m[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        bc += __shfl_xor_sync(0xffffffffu, bc, o);
+        bm += __shfl_xor_sync(0xffffffffu, bm, o);
+    }
+    c += bc;
+    m += bm;
+}
+
+__device__ __forceinline__ void sr_clear(SrShared& s)
+{
+    const int t = threadIdx.x;
+    s.cnt[t] = s.m0[t] = s.m1[t] = s.m2[t] = 0;
+}
+
+__device__ __forceinline__ void sr_add(SrShared& s, int bin, uint64_t mass)
+{
+    atomicAdd(&s.cnt[bin], 1u);
+    if (mass)
+    {
+        atomicAdd(&s.m0[bin], (uint32_t)(mass & 0x7FFF));
+        atomicAdd(&s.m1[bin], (uint32_t)((mass >> 15) & 0x7FFF));
+        atomicAdd(&s.m2[bin], (uint32_t)(mass >> 30));
+    }
+}
+
+// The row's totals of bin threadIdx.x over the cluster's histograms.
+template <int C>
+__device__ __forceinline__ void sr_collect(SrShared& s, uint32_t& c, uint64_t& m)
+{
+    const int t = threadIdx.x;
+    c = 0;
+    m = 0;
+    if constexpr (C == 1)
+    {
+        c = s.cnt[t];
+        m = (uint64_t)s.m0[t] + ((uint64_t)s.m1[t] << 15) + ((uint64_t)s.m2[t] << 30);
+    }
+    else
+    {
+        uint32_t v[C][4];
+#pragma unroll
+        for (int r = 0; r < C; ++r)
+        {
+            v[r][0] = peer_ld32(peer_addr(&s.cnt[t], r));
+            v[r][1] = peer_ld32(peer_addr(&s.m0[t], r));
+            v[r][2] = peer_ld32(peer_addr(&s.m1[t], r));
+            v[r][3] = peer_ld32(peer_addr(&s.m2[t], r));
+        }
+#pragma unroll
+        for (int r = 0; r < C; ++r)
+        {
+            c += v[r][0];
+            m += (uint64_t)v[r][1] + ((uint64_t)v[r][2] << 15) + ((uint64_t)v[r][3] << 30);
+        }
+    }
+}
+
+// C CTAs a row; E > 0: up to E logits of the slice per thread in registers,
+// E == 0: the slice is read again in every pass (from L2 after the first).
+template <int C, int E>
+__global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const SampleRowsArgs a)
+{
+    extern __shared__ __align__(16) uint8_t sr_raw[];
+    SrShared& s = *reinterpret_cast<SrShared*>(sr_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t row = blockIdx.x / C, rank = blockIdx.x % C;
+    const uint32_t per = (a.vocab + C - 1) / C;
+    const uint32_t v0 = rank * per, n_mine = v0 < a.vocab ? min(per, a.vocab - v0) : 0u;
+    const float* src = a.logits + (size_t)row * a.ld + v0;
+    const float NANF = __uint_as_float(0x7FC00000u);
+
+    float e[E > 0 ? E : 1];
+    if constexpr (E > 0)
+    {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+        {
+            const uint32_t j = (uint32_t)i * SR_THREADS + tid;
+            e[i] = j < n_mine ? __ldcs(src + j) : NANF;
+        }
+    }
+    // fn(logit, id) for each of this thread's tokens that is not NaN
+    auto each = [&](auto&& fn) {
+        if constexpr (E > 0)
+        {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (e[i] == e[i])
+                    fn(e[i], v0 + (uint32_t)i * SR_THREADS + tid);
+        }
+        else
+        {
+            for (uint32_t j = tid; j < n_mine; j += SR_THREADS)
+            {
+                const float l = src[j];
+                if (l == l)
+                    fn(l, v0 + j);
+            }
+        }
+    };
+
+    if (tid < 64)
+        s.tbl[tid] = exp2((double)tid / 64.0);
+    sr_clear(s);
+    // ---- the largest logit (its lowest id) and the smallest finite one
+    float mx = -INFINITY, mn = INFINITY;
+    uint32_t mi = 0xFFFFFFFFu;
+    each([&](float l, uint32_t id) {
+        if (l > mx || (l == mx && id < mi))
+        {
+            mx = l;
+            mi = id;
+        }
+        if (l > -INFINITY)
+            mn = fminf(mn, l);
+    });
+    auto better = [](float& v, uint32_t& i, float ov, uint32_t oi) {
+        if (ov > v || (ov == v && oi < i))
+        {
+            v = ov;
+            i = oi;
+        }
+    };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        better(mx, mi, __shfl_xor_sync(0xffffffffu, mx, o), __shfl_xor_sync(0xffffffffu, mi, o));
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if (lane == 0)
+    {
+        s.red_max[warp] = mx;
+        s.red_idx[warp] = mi;
+        s.red_min[warp] = mn;
+    }
+    __syncthreads();
+    mx = s.red_max[lane];
+    mi = s.red_idx[lane];
+    mn = s.red_min[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        better(mx, mi, __shfl_xor_sync(0xffffffffu, mx, o), __shfl_xor_sync(0xffffffffu, mi, o));
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if constexpr (C > 1)
+    {
+        if (tid == 0)
+        {
+            s.cta_max = mx;
+            s.cta_idx = mi;
+            s.cta_min = mn;
+        }
+        row_sync<C>();
+        mx = -INFINITY;
+        mi = 0xFFFFFFFFu;
+        mn = INFINITY;
+#pragma unroll
+        for (int r = 0; r < C; ++r)
+        {
+            better(mx, mi, __uint_as_float(peer_ld32(peer_addr(&s.cta_max, r))), peer_ld32(peer_addr(&s.cta_idx, r)));
+            mn = fminf(mn, __uint_as_float(peer_ld32(peer_addr(&s.cta_min, r))));
+        }
+    }
+    const float T = a.temperature ? a.temperature[row] : 1.0f;
+    if (!(T > 0.0f) || !isfinite(mx))
+    {
+        // greedy (T <= 0), or no finite logit to normalise by
+        if (rank == 0 && tid == 0)
+            a.tokens[row] = mi == 0xFFFFFFFFu ? 0u : mi;
+        row_sync<C>(); // no CTA leaves while another reads its shared memory
+        return;
+    }
+    SrRow R;
+    R.M = mx;
+    R.dM = (double)mx;
+    R.inv_t = 1.0 / (double)T;
+    const float mp = a.min_p ? a.min_p[row] : 0.0f;
+    R.min_p = mp > 0.0f ? fmin((double)mp, 1.0) : 0.0;
+    R.far = 33.0f * T; // exp(-33) is below half a unit
+    const float span = fminf(mx - mn, 40.0f * T);
+    R.invw = span > 0.0f ? (float)SR_BINS / span : 0.0f;
+
+    // ---- count and mass of the 1024 steps of M - l, then their prefix sums
+    __syncthreads();
+    each([&](float l, uint32_t) { sr_add(s, sr_bin(l, R), sr_mass(l, R, s.tbl)); });
+    row_sync<C>();
+    uint32_t c;
+    uint64_t m;
+    sr_collect<C>(s, c, m);
+    sr_scan(c, m, s);
+    s.pc[tid] = c;
+    s.pm[tid] = m;
+    row_sync<C>(); // the histograms are free again
+
+    // The first token whose cumulative count (by_count) or mass reaches the
+    // target: its order key and the mass up to and including it.
+    auto search = [&](bool by_count, uint32_t k, double target, uint64_t& key_out, uint64_t& mass_out) {
+        // one thread a step; hit: this step crosses the target
+        auto pick_step = [&](uint32_t c_incl, uint64_t m_incl, uint32_t c_excl, uint64_t m_excl) {
+            const bool in = by_count ? c_incl >= k : (c_incl > 0 && (double)m_incl >= target);
+            const bool before = by_count ? c_excl >= k : (c_excl > 0 && (double)m_excl >= target);
+            if (in && !before)
+            {
+                s.pick = tid;
+                s.above_c = c_excl;
+                s.above_m = m_excl;
+                s.n_in = c_incl - c_excl;
+            }
+        };
+        pick_step(s.pc[tid], s.pm[tid], tid ? s.pc[tid - 1] : 0u, tid ? s.pm[tid - 1] : 0ull);
+        if (tid == 0)
+            s.n_list = 0;
+        __syncthreads();
+        const int step = s.pick;
+        uint32_t above_c = s.above_c, n_in = s.n_in;
+        uint64_t above_m = s.above_m;
+        uint64_t prefix = 0;
+        int shift = 64; // the key bits from here up are fixed to prefix
+        row_sync<C>(); // n_list is zero in every CTA
+        while (n_in > (uint32_t)SR_LIST && shift > 0)
+        {
+            // narrow the step: the next 10 bits of the order key
+            const int nshift = shift > 10 ? shift - 10 : 0;
+            sr_clear(s);
+            __syncthreads();
+            each([&](float l, uint32_t id) {
+                const uint64_t key = order_key(l, id);
+                if (sr_bin(l, R) == step && (shift == 64 || (key >> shift) == (prefix >> shift)))
+                    sr_add(s, SR_BINS - 1 - (int)((key >> nshift) & ((1u << (shift - nshift)) - 1u)), sr_mass(l, R, s.tbl));
+            });
+            row_sync<C>();
+            uint32_t dc;
+            uint64_t dm;
+            sr_collect<C>(s, dc, dm);
+            const uint32_t own_c = dc;
+            const uint64_t own_m = dm;
+            sr_scan(dc, dm, s);
+            pick_step(above_c + dc, above_m + dm, above_c + dc - own_c, above_m + dm - own_m);
+            __syncthreads();
+            prefix |= (uint64_t)(SR_BINS - 1 - s.pick) << nshift;
+            shift = nshift;
+            above_c = s.above_c;
+            above_m = s.above_m;
+            n_in = s.n_in;
+            row_sync<C>();
+        }
+        // gather the step's tokens in the first CTA
+        each([&](float l, uint32_t id) {
+            if (sr_bin(l, R) == step)
+            {
+                const uint64_t key = order_key(l, id);
+                if (shift == 64 || (key >> shift) == (prefix >> shift))
+                {
+                    const uint64_t mass = sr_mass(l, R, s.tbl);
+                    if constexpr (C == 1)
+                    {
+                        const uint32_t at = atomicAdd(&s.n_list, 1u);
+                        if (at < (uint32_t)SR_LIST)
+                        {
+                            s.lkey[at] = key;
+                            s.lmass[at] = mass;
+                        }
+                    }
+                    else
+                    {
+                        const uint32_t at = peer_add32(peer_addr(&s.n_list, 0), 1u);
+                        if (at < (uint32_t)SR_LIST)
+                        {
+                            peer_st64(peer_addr(&s.lkey[at], 0), key);
+                            peer_st64(peer_addr(&s.lmass[at], 0), mass);
+                        }
+                    }
+                }
+            }
+        });
+        row_sync<C>();
+        if (rank == 0)
+        {
+            const uint32_t n = min(s.n_list, (uint32_t)SR_LIST);
+            if (tid < (int)n) // a token's place: how many keys are larger (keys are distinct)
+            {
+                const uint64_t key = s.lkey[tid];
+                uint32_t place = 0;
+                for (uint32_t j = 0; j < n; ++j)
+                    place += s.lkey[j] > key;
+                s.skey[place] = key;
+                s.smass[place] = s.lmass[tid];
+            }
+            __syncthreads();
+            uint32_t lc = tid < (int)n ? 1u : 0u;
+            uint64_t lm = tid < (int)n ? s.smass[tid] : 0ull;
+            const uint64_t own = lm;
+            sr_scan(lc, lm, s);
+            const bool in = by_count ? above_c + lc >= k : (double)(above_m + lm) >= target;
+            const bool before = tid == 0 ? false
+                                : by_count ? above_c + lc - 1 >= k
+                                           : (double)(above_m + lm - own) >= target;
+            if (tid < (int)n && ((in && !before) || (!in && tid == (int)n - 1)))
+            {
+#pragma unroll
+                for (int r = 0; r < C; ++r)
+                {
+                    if constexpr (C == 1)
+                    {
+                        s.found_key = s.skey[tid];
+                        s.found_mass = above_m + lm;
+                    }
+                    else
+                    {
+                        peer_st64(peer_addr(&s.found_key, r), s.skey[tid]);
+                        peer_st64(peer_addr(&s.found_mass, r), above_m + lm);
+                    }
+                }
+            }
+        }
+        row_sync<C>();
+        key_out = s.found_key;
+        mass_out = s.found_mass;
+    };
+
+    uint64_t key, W = s.pm[SR_BINS - 1];
+    const int k = a.top_k ? a.top_k[row] : 0;
+    if (k > 0 && (uint32_t)k < s.pc[SR_BINS - 1])
+        search(true, (uint32_t)k, 0.0, key, W);
+    const float tp = a.top_p ? a.top_p[row] : 1.0f;
+    if (tp < 1.0f)
+        search(false, 0, (double)tp * (double)W, key, W);
+    const float uu = a.u[row];
+    search(false, 0, uu > 0.0f ? fmin((double)uu, 1.0) * (double)W : 0.0, key, W);
+    if (rank == 0 && tid == 0)
+        a.tokens[row] = 0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFu);
+    row_sync<C>();
+}
+
+template <int C, int E>
+int sr_launch(const SampleRowsArgs& a, cudaStream_t st)
+{
+    static PerDeviceOnce attrs;
+    const int arc = attrs.run([]() -> int {
+        AAEDN_CUDA_TRY(cudaFuncSetAttribute(sample_rows_kernel<C, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)sizeof(SrShared)));
+        return AAEDN_OK;
+    });
+    if (arc)
+        return arc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.rows * C);
+    cfg.blockDim = dim3(SR_THREADS);
+    cfg.dynamicSmemBytes = sizeof(SrShared);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_rows_kernel<C, E>, a);
+    if (e != cudaSuccess)
+        return set_error(AAEDN_ECUDA, "launch of sample_rows_kernel failed: %s", cudaGetErrorString(e));
+    count_launch();
+    return AAEDN_OK;
+}
+
+template <int C>
+int sr_launch_e(const SampleRowsArgs& a, cudaStream_t st)
+{
+    const uint32_t per = (a.vocab + C - 1) / C;
+    if (per <= 8u * SR_THREADS)
+        return sr_launch<C, 8>(a, st);
+    if (per <= 16u * SR_THREADS)
+        return sr_launch<C, 16>(a, st);
+    if (per <= 32u * SR_THREADS)
+        return sr_launch<C, 32>(a, st);
+    return sr_launch<C, 0>(a, st);
+}
+
+} // namespace
+
+int sample_rows(const SampleRowsArgs& a, cudaStream_t st)
+{
+    // the fewest CTAs a row whose registers hold it (32 logits a thread),
+    // then more while the rows leave SMs idle and a CTA has over 2048 tokens
+    int C = 1;
+    while (C < 8 && (a.vocab + C - 1) / C > 32u * SR_THREADS)
+        C *= 2;
+    while (C < 8 && (size_t)a.rows * C * 2 <= (size_t)sm_count() && (a.vocab + C - 1) / C > 2048)
+        C *= 2;
+    switch (C)
+    {
+    case 1: return sr_launch_e<1>(a, st);
+    case 2: return sr_launch_e<2>(a, st);
+    case 4: return sr_launch_e<4>(a, st);
+    default: return sr_launch_e<8>(a, st);
+    }
+}
+
+} // namespace aaedn_dev
+
+using namespace aaedn_dev;
+
+extern "C" int aaedn_cu_sample_rows(const float* d_logits, size_t ld, size_t rows, uint32_t vocab,
+                                    const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
+                                    const float* d_min_p, const float* d_u, uint32_t* d_tokens, void* stream)
+{
+    const char* fn = "aaedn_cu_sample_rows";
+    if (rows == 0)
+        return AAEDN_OK;
+    if (vocab == 0 || vocab > SR_MAX_VOCAB)
+        return set_error(AAEDN_EINVAL, "%s: vocab %u outside 1..%u", fn, vocab, SR_MAX_VOCAB);
+    if (rows > ((size_t)1 << 24) || ld < vocab)
+        return set_error(AAEDN_EINVAL, "%s: at most 2^24 rows (%zu), ld %zu at least vocab", fn, rows, ld);
+    if (!d_logits || !d_u || !d_tokens)
+        return set_error(AAEDN_EINVAL, "%s: %s is null", fn, !d_logits ? "d_logits" : !d_u ? "d_u" : "d_tokens");
+    int rc;
+    if ((rc = check_device_ptr(fn, d_logits, "d_logits", 4)) || (rc = check_device_ptr(fn, d_u, "d_u", 4)) ||
+        (rc = check_device_ptr(fn, d_tokens, "d_tokens", 4)) ||
+        (d_temperature && (rc = check_device_ptr(fn, d_temperature, "d_temperature", 4))) ||
+        (d_top_k && (rc = check_device_ptr(fn, d_top_k, "d_top_k", 4))) ||
+        (d_top_p && (rc = check_device_ptr(fn, d_top_p, "d_top_p", 4))) ||
+        (d_min_p && (rc = check_device_ptr(fn, d_min_p, "d_min_p", 4))))
+        return rc;
+    SampleRowsArgs a{};
+    a.logits = d_logits;
+    a.ld = ld;
+    a.rows = (uint32_t)rows;
+    a.vocab = vocab;
+    a.temperature = d_temperature;
+    a.top_k = d_top_k;
+    a.top_p = d_top_p;
+    a.min_p = d_min_p;
+    a.u = d_u;
+    a.tokens = d_tokens;
+    return sample_rows(a, as_stream(stream));
+}
