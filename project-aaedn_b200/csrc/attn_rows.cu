@@ -1,6 +1,7 @@
 // attn_rows.cu — attention of packed query rows over the paged fp32 K/V cache
 // (the sequences of a batch in one call), causal or under a tree mask, and
 // its C ABI.
+#include <algorithm>
 #include <climits>
 
 #include "common.cuh"
@@ -46,6 +47,13 @@ __device__ __forceinline__ const int* rows_page_table(const AttnRowsArgs& a, int
 {
     return a.page_table + (size_t)(a.seq_of ? a.seq_of[s] : s) * a.pt_stride;
 }
+
+} // namespace aaedn_dev
+
+#include "attn_rows_tc.cuh"
+
+namespace aaedn_dev
+{
 
 // ---------------------------------------------------------------------------
 // One warp per (packed row, query head), every head_dim (a multiple of 4, at
@@ -145,10 +153,62 @@ __global__ void __launch_bounds__(RW_WARPS * 32) attn_rows_warp_kernel(const Att
             o[lane + 32 * i] = acc[i] * inv;
 }
 
-int attn_rows_init() { return AAEDN_OK; }
+template <int HDP, bool TREE>
+static int rows_tc_attrs()
+{
+    auto kern = attn_rows_tc_kernel<HDP, TREE>;
+    AAEDN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RtCfg<HDP>::SMEM));
+    cudaFuncAttributes at;
+    AAEDN_CUDA_TRY(cudaFuncGetAttributes(&at, kern));
+    if (at.numRegs != RT_REGS) // the roles' register shares are drawn from the launch's
+        return set_error(AAEDN_EUNSUPPORTED, "attn_rows_tc_kernel built with %d registers, not %d", at.numRegs, RT_REGS);
+    return AAEDN_OK;
+}
+
+int attn_rows_init()
+{
+    static PerDeviceOnce once;
+    return once.run([]() -> int {
+        int rc;
+        if ((rc = rows_tc_attrs<64, false>()) || (rc = rows_tc_attrs<64, true>()) || (rc = rows_tc_attrs<128, false>()))
+            return rc;
+        return rows_tc_attrs<128, true>();
+    });
+}
+
+template <int HDP, bool TREE>
+static int rows_tc_launch(const AttnRowsArgs& a, cudaStream_t st)
+{
+    unsigned* err = a.err;
+    if (!err)
+    {
+        void* p = nullptr;
+        AAEDN_CUDA_TRY(cudaGetSymbolAddress(&p, g_attn_rows_err));
+        err = static_cast<unsigned*>(p);
+    }
+    // one CTA an SM, as far as the workspace's partial sums go
+    const int grid = std::min<int>(sm_count(), (int)((AAEDN_ATTN_ROWS_WORKSPACE_BYTES - RT_HEADER_BYTES) /
+                                                     (2 * rt_slot_bytes<HDP>())));
+    attn_rows_tc_kernel<HDP, TREE><<<grid, RT_THREADS, RtCfg<HDP>::SMEM, st>>>(a, err);
+    AAEDN_LAUNCH_CHECK("attn_rows_tc_kernel");
+    const cudaError_t e = launch_kernel(attn_rows_join_kernel<HDP, TREE>, dim3((unsigned)grid - 1, 128 / RJ_WARPS),
+                                        dim3(RJ_WARPS * 32), 0, st, true, a, grid);
+    if (e != cudaSuccess)
+        return set_error(AAEDN_ECUDA, "launch of attn_rows_join_kernel failed: %s", cudaGetErrorString(e));
+    count_launch();
+    return AAEDN_OK;
+}
 
 int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
 {
+    if (a.head_dim <= 128)
+    {
+        if (int rc = attn_rows_init())
+            return rc;
+        if (a.head_dim <= 64)
+            return a.mask ? rows_tc_launch<64, true>(a, st) : rows_tc_launch<64, false>(a, st);
+        return a.mask ? rows_tc_launch<128, true>(a, st) : rows_tc_launch<128, false>(a, st);
+    }
     const dim3 grid((unsigned)((a.rows + RW_WARPS - 1) / RW_WARPS), (unsigned)a.n_heads);
     if (a.mask)
         attn_rows_warp_kernel<true><<<grid, RW_WARPS * 32, 0, st>>>(a);

@@ -1,0 +1,1066 @@
+// attn_rows_tc.cuh — attention of packed query rows over the paged fp32 K/V
+// cache on the 5th-generation tensor cores (head_dim up to 128).
+//
+// Tile: 128 query rows that share a K/V head (128 / G tokens x the G query
+// heads of the K/V head) against the keys in units of one page (64 tokens):
+// S = Q K^T (M 128, N 64), online softmax, O += P V (M 128, N head_dim). The
+// Q and P operands and the accumulators are in tensor memory, K and V in
+// shared memory.
+//
+// Precision: the cache is fp32, the MMA takes 16-bit factors. A factor x is
+// carried as x_hi + x_lo, both fp16, of x scaled by a power of two (q: per
+// row, K and V: per unit, P: by 2^14) that puts the largest magnitude at
+// 2^14..2^15: 22 significant bits for magnitudes down to 2^-28 of the
+// largest, an absolute 2^-39 of it below. Each product is three MMAs (hi lo,
+// lo hi, hi hi; lo lo is below 2^-22 of it), the small ones first, so that
+// the tensor core's rounding of its accumulator (up to one unit per MMA)
+// only counts for the hi hi ones. bf16 would need six products for this, and
+// TF32 three at half the rate. P V accumulates one unit in tensor memory and
+// is added to fp32 registers (one rounding a unit, with the softmax
+// correction), because a long chain of tensor-core additions is biased
+// towards zero: 2^-24 each.
+//
+// Work split: the units of all (sequence, K/V head, tile) in a row are cut
+// into equal shares, one persistent CTA each, so long prompts, many short
+// ones and a small tree over a long cache all fill the GPU. A tile that a cut
+// goes through is written as partial sums (at most two a CTA) that a second
+// kernel joins, in a fixed order: no atomics, the same bits every time.
+//
+// Roles (20 warps, 1 CTA an SM): warp 0 copies pages (bulk copies into a ring
+// of stages), warp 1 issues the MMAs; warps 4-7 softmax (one row a thread:
+// S from tensor memory, P back over it); warps 8-11 the output sums (one row
+// a thread, in registers); warps 12-19 turn a stage from fp32 into the two
+// fp16 parts in place, in the 128-byte-swizzled layout the MMA reads (rows =
+// keys: K-major for K, the same bytes are MN-major for V). Ring order is the
+// MMA's: K0, K1, V0, K2, V1, ..., so S of the next unit is computed while the
+// softmax of this one runs.
+//
+// Keys that do not exist (behind the cached tokens, in a page outside the
+// pool) are zeros that every row masks; a non-finite K or V row is replaced
+// by zeros and noted, and the rows that attend it become NaN, so it cannot
+// reach the other rows of the tile through 0 * NaN.
+#pragma once
+
+#include "attn_rows.h"
+#include "common.cuh"
+
+namespace aaedn_dev
+{
+
+constexpr int RT_WARPS = 20, RT_THREADS = RT_WARPS * 32;
+constexpr int RT_CONV_THREADS = 256;
+constexpr int RT_REGS = 96; // registers a thread at launch: 65536 / 640, whole eights
+// the warpgroups' shares after setmaxnreg: together the launch's
+constexpr int RT_REGS_IO = 48, RT_REGS_SM = 120, RT_REGS_O = 184, RT_REGS_CV = 64;
+static_assert(RT_REGS_IO + RT_REGS_SM + RT_REGS_O + 2 * RT_REGS_CV == 5 * RT_REGS, "register shares");
+constexpr uint64_t RT_WAIT_LIMIT_NS = 2000000000ull;
+constexpr int RT_INFO = 16; // units whose scales are kept
+
+// tensor memory columns
+constexpr uint32_t RT_T_S = 0, RT_T_O = 128, RT_T_Q = 384, RT_T_QLO = 64, RT_T_COLS = 512;
+
+template <int HDP> // head_dim rounded up to whole 64
+struct RtCfg
+{
+    static constexpr int NS = HDP == 128 ? 6 : 8; // stages of one page of K or V
+    static constexpr uint32_t STAGE = 64u * HDP * 4u;
+    static constexpr int NB = HDP / 64;
+    static constexpr size_t SMEM = (size_t)NS * STAGE + 1024; // + alignment slack
+};
+
+// ---- the split of the work ----------------------------------------------------
+// sum over i < n of floor((a i + b) / 64)
+__host__ __device__ inline unsigned long long rt_floor_sum(unsigned long long n, unsigned long long a,
+                                                           unsigned long long b)
+{
+    unsigned long long m = 64, r = 0;
+    while (true)
+    {
+        if (a >= m)
+        {
+            r += n * (n - 1) / 2 * (a / m);
+            a %= m;
+        }
+        if (b >= m)
+        {
+            r += n * (b / m);
+            b %= m;
+        }
+        const unsigned long long y = a * n + b;
+        if (y < m)
+            return r;
+        n = y / m;
+        b = y % m;
+        const unsigned long long t = m;
+        m = a;
+        a = t;
+    }
+}
+
+struct RtSeq
+{
+    int begin, n, past; // first packed row, rows, cached tokens
+    int tiles;          // tiles of R tokens
+    int cap, nodes;     // slots the table has; tree: mask bits that count
+};
+
+__host__ __device__ inline int rt_keys(const RtSeq& q, bool tree, int R, int tile)
+{
+    const int last = tree ? q.nodes : (tile + 1 < q.tiles ? (tile + 1) * R : q.n);
+    const long long k = (long long)q.past + last;
+    return k < q.cap ? (int)k : q.cap;
+}
+
+// units of the first `tiles` tiles of one K/V head
+__host__ __device__ inline unsigned long long rt_units_before(const RtSeq& q, bool tree, int R, int tiles)
+{
+    if (tiles <= 0)
+        return 0;
+    if (tree)
+        return (unsigned long long)tiles * ((rt_keys(q, true, R, 0) + 63) / 64);
+    unsigned long long full = (unsigned long long)(tiles < q.tiles ? tiles : q.tiles - 1), sum = 0;
+    // tile i < full sees past + (i + 1) R keys, at most cap
+    unsigned long long below = 0; // tiles under the cap
+    if (q.cap > q.past)
+        below = (unsigned long long)(q.cap - q.past) / (unsigned)R;
+    if (below > full)
+        below = full;
+    if (below)
+        sum += rt_floor_sum(below, (unsigned)R, (unsigned long long)q.past + (unsigned)R + 63);
+    sum += (full - below) * (((unsigned long long)q.cap + 63) / 64);
+    if (tiles >= q.tiles)
+        sum += (rt_keys(q, false, R, q.tiles - 1) + 63) / 64;
+    return sum;
+}
+
+__device__ __forceinline__ RtSeq rt_seq(const AttnRowsArgs& a, int s, int R)
+{
+    RtSeq q;
+    q.begin = min(max(a.row_start[s], 0), a.rows);
+    const int end = min(max(a.row_start[s + 1], q.begin), a.rows);
+    q.n = end - q.begin;
+    q.past = max(a.past[s], 0);
+    q.tiles = (q.n + R - 1) / R;
+    q.cap = (int)(a.pt_stride * ROWS_PAGE); // pt_stride <= 2^24
+    q.nodes = min(q.n, a.mask_words * 64);
+    return q;
+}
+
+// Where a CTA starts (also what the joining kernel reads).
+struct RtStart
+{
+    int s, h, t, u;            // sequence, K/V head, tile, unit in the tile
+    unsigned long long begin;  // first unit of the CTA's share
+    unsigned long long total;  // units of the call
+};
+
+constexpr size_t RT_HEADER_BYTES = 64 * 1024;
+// partial sums: [CTA][2][128 rows][HDP], then [CTA][2][128 rows] (sum, offset)
+template <int HDP>
+__host__ __device__ inline size_t rt_slot_bytes()
+{
+    return (size_t)128 * HDP * 4 + 128 * 8;
+}
+template <int HDP>
+__device__ __forceinline__ float* rt_slot(const AttnRowsArgs& a, int cta, int which)
+{
+    return reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + RT_HEADER_BYTES +
+                                    (size_t)(cta * 2 + which) * rt_slot_bytes<HDP>());
+}
+
+__device__ __forceinline__ unsigned long long rt_share(unsigned long long total, int cta, int grid)
+{
+    return total * (unsigned)cta / (unsigned)grid;
+}
+
+// The position of unit `at` (one warp; the result in every lane).
+template <bool TREE>
+__device__ RtStart rt_locate(const AttnRowsArgs& a, int R, int cta, int grid)
+{
+    const int lane = threadIdx.x & 31;
+    auto units_of = [&](int s) -> unsigned long long {
+        if (s >= a.n_seqs)
+            return 0;
+        const RtSeq q = rt_seq(a, s, R);
+        return q.n ? (unsigned long long)a.n_kv * rt_units_before(q, TREE, R, q.tiles) : 0;
+    };
+    unsigned long long total = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
+        total += units_of(s0 + lane);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    RtStart r{};
+    r.total = total;
+    r.begin = rt_share(total, cta, grid);
+    unsigned long long before = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
+    {
+        const unsigned long long mine = units_of(s0 + lane);
+        unsigned long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o)
+                incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > r.begin);
+        if (hit)
+        {
+            const int l = __ffs(hit) - 1;
+            r.s = s0 + l;
+            unsigned long long off = r.begin - before - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, mine, l));
+            const RtSeq q = rt_seq(a, r.s, R);
+            const unsigned long long per = rt_units_before(q, TREE, R, q.tiles);
+            r.h = (int)(off / per);
+            off -= per * (unsigned)r.h;
+            int lo = 0, hi = q.tiles - 1; // the last tile with units_before(tile) <= off
+            while (lo < hi)
+            {
+                const int mid = (lo + hi + 1) >> 1;
+                if (rt_units_before(q, TREE, R, mid) <= off)
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            r.t = lo;
+            r.u = (int)(off - rt_units_before(q, TREE, R, lo));
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return r;
+}
+
+// A CTA's items in order: (sequence, K/V head, tile) with units [u0, u1).
+template <bool TREE>
+struct RtCursor
+{
+    RtSeq q;
+    int s, h, t, u0, u1, keys;
+    bool whole; // the item has every unit of its tile
+    unsigned long long left;
+
+    __device__ __forceinline__ void set(int R)
+    {
+        keys = rt_keys(q, TREE, R, t);
+        const int units = (keys + 63) / 64;
+        u1 = (unsigned long long)(units - u0) <= left ? units : u0 + (int)left;
+        whole = u0 == 0 && u1 == units;
+    }
+    // the first item; false: the CTA has none
+    __device__ __forceinline__ bool start(const AttnRowsArgs& a, const RtStart& st, unsigned long long share, int R)
+    {
+        left = share;
+        if (!left)
+            return false;
+        s = st.s;
+        h = st.h;
+        t = st.t;
+        u0 = st.u;
+        q = rt_seq(a, s, R);
+        set(R);
+        return true;
+    }
+    __device__ __forceinline__ bool next(const AttnRowsArgs& a, int R)
+    {
+        left -= (unsigned)(u1 - u0);
+        if (!left)
+            return false;
+        u0 = 0;
+        if (++t >= q.tiles)
+        {
+            t = 0;
+            if (++h >= a.n_kv)
+            {
+                h = 0;
+                do
+                {
+                    if (++s >= a.n_seqs)
+                        return false; // the arrays changed under the kernel
+                    q = rt_seq(a, s, R);
+                } while (q.n == 0);
+            }
+        }
+        set(R);
+        return true;
+    }
+};
+
+// ---- tensor memory ------------------------------------------------------------
+__device__ __forceinline__ void rt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void rt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void rt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of the warp's 32 lanes; the registers hold them after the wait.
+__device__ __forceinline__ void rt_ld32(uint32_t taddr, float* v)
+{
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void rt_st8(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+// D[tensor memory] (+)= A[tensor memory] B[shared memory], fp16 in, fp32 out
+__device__ __forceinline__ void rt_mma(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+
+__device__ __forceinline__ void rt_commit(uint32_t mbar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
+}
+
+// Shared-memory descriptors of the 128-byte-swizzled operand. K: rows = keys,
+// K-major, 8-key groups 1024 bytes apart. V: the same bytes as an MN-major
+// operand: 64-dim blocks 8192 bytes apart (leading offset), 8-key groups
+// 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t rt_desc(uint32_t saddr, uint32_t lead)
+{
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+// kind::f16 with fp16 A and B, fp32 D, M = 128; b_mn: B is MN-major
+__host__ __device__ constexpr uint32_t rt_idesc(int n, bool b_mn)
+{
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ float rt_exp2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ float2 rt_add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 pa, pb, pd;\n\tmov.b64 pa, {%2, %3};\n\tmov.b64 pb, {%4, %5};\n\t"
+        "add.rn.f32x2 pd, pa, pb;\n\tmov.b64 {%0, %1}, pd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// x and y as their fp16 high and low parts (pairs, x in the low half)
+__device__ __forceinline__ void rt_split2(float x, float y, uint32_t& hi, uint32_t& lo)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 hf = __half22float2(h);
+    const float2 r = fma2_rn(hf, make_float2(-1.0f, -1.0f), make_float2(x, y)); // exact
+    const __half2 l = __floats2half2_rn(r.x, r.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// The power of two that puts a magnitude with these bits at 2^14..2^15, and
+// its inverse (both normal numbers).
+__device__ __forceinline__ void rt_scale_of(uint32_t max_bits, float& up, float& down)
+{
+    const int e = min(141 - (int)(max_bits >> 23), 126);
+    const int k = max_bits ? max(e, -113) : 0;
+    up = __uint_as_float((uint32_t)(k + 127) << 23);
+    down = __uint_as_float((uint32_t)(127 - k) << 23);
+}
+
+template <int REGS>
+__device__ __forceinline__ void rt_regs_inc()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void rt_regs_dec()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+struct RtUnitInfo
+{
+    float k_down, v_down;      // what undoes the unit's scaling of K and V
+    int valid;                 // keys of the unit that exist
+    uint32_t kbad[2], vbad[2]; // keys with a non-finite K / V value
+};
+
+struct RtShared
+{
+    uint64_t raw[8], conv[8], free_[8]; // per stage: copied, converted, read by the MMAs
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
+    uint32_t tmem, abort;
+    RtStart start;
+    int stage_valid[8];
+    uint32_t wmax[2][8];
+    RtUnitInfo info[RT_INFO];
+    float alpha[4][128];
+    float2 stats[4][128]; // (sum, offset) of an item's rows
+};
+
+// Which of the 64 keys of a unit a row attends. limit: causal: the row's last
+// slot; tree: past. nodes: tree: the sequence's nodes (mask bits that count).
+template <bool TREE>
+__device__ __forceinline__ uint64_t rt_seen(int u, int valid, int limit, const uint64_t* mask, int words)
+{
+    uint64_t m;
+    const int base = u * 64;
+    if (!TREE)
+    {
+        const int lim = limit - base; // keys 0..lim
+        m = lim >= 63 ? ~0ull : lim < 0 ? 0ull : (2ull << lim) - 1;
+    }
+    else
+    {
+        const int d = base - limit; // node of the unit's first key
+        if (d <= -64)
+            m = ~0ull;
+        else if (d < 0)
+            m = ((1ull << -d) - 1) | (mask[0] << -d);
+        else
+        {
+            const int w = d >> 6, sh = d & 63;
+            m = w < words ? mask[w] >> sh : 0ull;
+            if (sh && w + 1 < words)
+                m |= mask[w + 1] << (64 - sh);
+        }
+    }
+    return valid >= 64 ? m : valid <= 0 ? 0ull : m & ((1ull << valid) - 1);
+}
+
+// ---------------------------------------------------------------------------
+template <int HDP, bool TREE>
+__global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnRowsArgs a, unsigned* err)
+{
+    using Cfg = RtCfg<HDP>;
+    constexpr int NS = Cfg::NS, NB = Cfg::NB;
+    extern __shared__ __align__(16) uint8_t rt_raw[];
+    __shared__ RtShared sm;
+    const uint32_t ring = (smem_addr(rt_raw) + 1023u) & ~1023u; // the swizzle works on address bits
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = a.n_heads / a.n_kv, R = 128 / G, hd = a.head_dim;
+    volatile uint32_t* abort = &sm.abort;
+
+    auto stage_at = [&](uint32_t pos) { return ring + (pos % NS) * Cfg::STAGE; };
+    auto bar_raw = [&](uint32_t pos) { return smem_addr(&sm.raw[pos % NS]); };
+    auto bar_conv = [&](uint32_t pos) { return smem_addr(&sm.conv[pos % NS]); };
+    auto bar_free = [&](uint32_t pos) { return smem_addr(&sm.free_[pos % NS]); };
+    auto phase = [&](uint32_t pos) { return (pos / NS) & 1u; };
+    auto fail = [&]() {
+        *abort = 1u;
+        atomicExch(err, 1u);
+    };
+    // bounded; gives up at once when another role gave up
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        if (mbar_try_wait(bar, parity))
+            return true;
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(bar, parity))
+        {
+            if (*abort)
+                return false;
+            if (globaltimer_ns() - t0 > RT_WAIT_LIMIT_NS)
+            {
+                fail();
+                return false;
+            }
+        }
+        return true;
+    };
+
+    if (warp == 0)
+    {
+        const RtStart st = rt_locate<TREE>(a, R, blockIdx.x, gridDim.x);
+        if (lane == 0)
+        {
+            sm.start = st;
+            reinterpret_cast<RtStart*>(a.workspace)[blockIdx.x] = st;
+        }
+    }
+    else if (warp == 1)
+    {
+        if (lane == 0)
+        {
+            for (int i = 0; i < 8; ++i)
+            {
+                mbar_init(smem_addr(&sm.raw[i]), 1);
+                mbar_init(smem_addr(&sm.conv[i]), RT_CONV_THREADS / 32);
+                mbar_init(smem_addr(&sm.free_[i]), 1);
+            }
+            for (int i = 0; i < 2; ++i)
+            {
+                mbar_init(smem_addr(&sm.s_full[i]), 1);
+                mbar_init(smem_addr(&sm.p_full[i]), 4);
+                mbar_init(smem_addr(&sm.o_full[i]), 1);
+                mbar_init(smem_addr(&sm.o_empty[i]), 4);
+            }
+            mbar_init(smem_addr(&sm.q_full), 4);
+            mbar_init(smem_addr(&sm.done), 1);
+            mbar_init_fence();
+            sm.abort = 0u;
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)),
+                     "r"(RT_T_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    else if (warp == 2 && lane < RT_INFO)
+    {
+        sm.info[lane].kbad[0] = sm.info[lane].kbad[1] = 0u;
+        sm.info[lane].vbad[0] = sm.info[lane].vbad[1] = 0u;
+    }
+    rt_fence_before();
+    __syncthreads();
+    rt_fence_after();
+    const uint32_t tmem = sm.tmem;
+    const RtStart st0 = sm.start;
+    const unsigned long long share = rt_share(st0.total, blockIdx.x + 1, gridDim.x) - st0.begin;
+
+    if (warp < 4)
+    {
+        rt_regs_dec<RT_REGS_IO>();
+        if (warp == 0)
+        {
+            // ---- producer: K0, K1, V0, K2, V1, ... of every item
+            uint32_t pos = 0;
+            bool ok = true;
+            auto emit = [&](const float* pool, int page, int h, int valid) {
+                // lane 0; a page outside the pool is a unit without keys
+                if (pos >= NS && !wait(bar_free(pos), phase(pos) ^ 1u))
+                    return false;
+                const bool there = page >= 0 && page < a.n_pages;
+                sm.stage_valid[pos % NS] = there ? valid : 0;
+                if (there)
+                {
+                    const uint32_t bytes = (uint32_t)valid * hd * 4u;
+                    mbar_arrive_expect_tx(bar_raw(pos), bytes);
+                    bulk_g2s(stage_at(pos), pool + ((size_t)page * a.n_kv + h) * (size_t)(ROWS_PAGE * hd), bytes,
+                             bar_raw(pos));
+                }
+                else
+                    mbar_arrive(bar_raw(pos));
+                ++pos;
+                return true;
+            };
+            RtCursor<TREE> c;
+            int vpage = 0, vh = 0, vvalid = 0; // the V that is due
+            bool due = false;
+            for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R))
+            {
+                const int* pt = rows_page_table(a, c.s);
+                for (int u0 = c.u0; u0 < c.u1 && ok; u0 += 32)
+                {
+                    const int mine = u0 + lane < c.u1 ? __ldg(pt + u0 + lane) : 0;
+                    for (int u = u0; u < min(u0 + 32, c.u1) && ok; ++u)
+                    {
+                        const int page = __shfl_sync(0xffffffffu, mine, u - u0);
+                        const int valid = min(64, c.keys - u * 64);
+                        if (lane == 0)
+                        {
+                            if (u == c.u0 && due)
+                                ok = emit(a.v, vpage, vh, vvalid);
+                            if (ok)
+                                ok = emit(a.k, page, c.h, valid);
+                            if (ok && u > c.u0)
+                                ok = emit(a.v, vpage, vh, vvalid);
+                        }
+                        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                        vpage = page;
+                        vh = c.h;
+                        vvalid = valid;
+                        due = true;
+                    }
+                }
+            }
+            if (lane == 0)
+            {
+                if (ok && due)
+                    emit(a.v, vpage, vh, vvalid);
+                // the copies it issued have landed before the CTA may exit
+                for (uint32_t p = pos > NS ? pos - NS : 0; p < pos; ++p)
+                    mbar_wait_bounded(bar_raw(p), phase(p), RT_WAIT_LIMIT_NS);
+            }
+            __syncwarp();
+        }
+        else if (warp == 1)
+        {
+            // ---- MMA issuer (one thread)
+            if (lane == 0)
+            {
+                constexpr uint32_t id_qk = rt_idesc(64, false), id_pv = rt_idesc(HDP, true);
+                uint32_t pos = 0, g = 0, item = 0;
+                bool ok = true;
+                auto qk = [&](bool first) {
+                    if (first && !wait(smem_addr(&sm.q_full), item & 1u))
+                        return false;
+                    if (!wait(bar_conv(pos), phase(pos)))
+                        return false;
+                    rt_fence_after();
+                    const uint32_t d = tmem + RT_T_S + (g & 1u) * 64u, kb = stage_at(pos);
+                    const uint32_t qh = tmem + RT_T_Q, ql = qh + (HDP == 128 ? RT_T_QLO : 32u);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) // q_hi k_lo, q_lo k_hi, q_hi k_hi
+#pragma unroll
+                        for (int k = 0; k < HDP / 16; ++k)
+                            rt_mma(d, (p == 1 ? ql : qh) + k * 8,
+                                   rt_desc(kb + (p == 0 ? NB * 8192u : 0u) + (k >> 2) * 8192u + (k & 3) * 32u, 16u), id_qk,
+                                   (p | k) != 0 ? 1u : 0u);
+                    rt_commit(smem_addr(&sm.s_full[g & 1u]));
+                    rt_commit(bar_free(pos));
+                    ++pos;
+                    return true;
+                };
+                auto pv = [&](uint32_t j) { // unit j
+                    if (!wait(bar_conv(pos), phase(pos)) || !wait(smem_addr(&sm.p_full[j & 1u]), (j >> 1) & 1u) ||
+                        (j >= 2 && !wait(smem_addr(&sm.o_empty[j & 1u]), ((j >> 1) & 1u) ^ 1u)))
+                        return false;
+                    rt_fence_after();
+                    const uint32_t d = tmem + RT_T_O + (j & 1u) * 128u, vb = stage_at(pos);
+                    const uint32_t ph = tmem + RT_T_S + (j & 1u) * 64u, pl = ph + 32u;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            rt_mma(d, (p == 1 ? pl : ph) + k * 8,
+                                   rt_desc(vb + (p == 0 ? NB * 8192u : 0u) + k * 2048u, 8192u), id_pv, (p | k) != 0 ? 1u : 0u);
+                    rt_commit(smem_addr(&sm.o_full[j & 1u]));
+                    rt_commit(bar_free(pos));
+                    ++pos;
+                    return true;
+                };
+                RtCursor<TREE> c;
+                for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
+                    for (int u = c.u0; u < c.u1 && ok; ++u, ++g)
+                    {
+                        if (u == c.u0 && g > 0)
+                            ok = pv(g - 1);
+                        ok = ok && qk(u == c.u0);
+                        if (ok && u > c.u0)
+                            ok = pv(g - 1);
+                    }
+                if (ok && g > 0)
+                    pv(g - 1);
+                rt_commit(smem_addr(&sm.done)); // every MMA issued, whatever happened
+            }
+            __syncwarp();
+        }
+    }
+    else if (warp < 8)
+    {
+        // ---- softmax: thread = row
+        rt_regs_inc<RT_REGS_SM>();
+        const int i = (warp & 3) * 32 + lane, ti = i / G, gi = i - ti * G;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        constexpr float LOG2E = 1.4426950408889634f;
+        const float qs = fabsf(a.scale) * LOG2E, sign = a.scale < 0.0f ? -1.0f : 1.0f;
+        uint32_t g = 0, item = 0;
+        bool ok = true;
+        RtCursor<TREE> c;
+        for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
+        {
+            // the row's query into tensor memory (every product with the last
+            // item's is done: its last S was waited for)
+            const int r = c.t * R + ti;
+            const bool live = ti < R && r < c.q.n;
+            const float4* qr = reinterpret_cast<const float4*>(a.q + (size_t)(c.q.begin + (live ? r : 0)) * a.ldq +
+                                                               (size_t)(c.h * G + gi) * hd);
+            uint32_t mb = 0;
+            if (live)
+#pragma unroll 8
+                for (int d = 0; d < HDP / 4; ++d)
+                    if (d * 4 < hd)
+                    {
+                        const float4 x = qr[d];
+                        mb = max(max(mb, max(__float_as_uint(x.x) & 0x7FFFFFFFu, __float_as_uint(x.y) & 0x7FFFFFFFu)),
+                                 max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu));
+                    }
+            float q_up, q_down;
+            rt_scale_of(mb, q_up, q_down);
+            q_up *= sign;
+#pragma unroll
+            for (int d0 = 0; d0 < HDP / 16; ++d0)
+            {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                {
+                    const float4 x = live && (d0 * 4 + d) * 4 < hd ? qr[d0 * 4 + d] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    rt_split2(x.x * q_up, x.y * q_up, hi[2 * d], lo[2 * d]);
+                    rt_split2(x.z * q_up, x.w * q_up, hi[2 * d + 1], lo[2 * d + 1]);
+                }
+                rt_st8(tmem + lanes + RT_T_Q + d0 * 8, hi);
+                rt_st8(tmem + lanes + RT_T_Q + (HDP == 128 ? RT_T_QLO : 32u) + d0 * 8, lo);
+            }
+            rt_wait_st();
+            rt_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(smem_addr(&sm.q_full));
+            const float qf = qs * q_down;
+            const int limit = TREE ? c.q.past : min(c.q.past, INT_MAX - c.q.n) + r; // past + r: far behind cap when clamped
+            const uint64_t* mask = TREE ? a.mask + (size_t)(c.q.begin + (live ? r : 0)) * a.mask_words : nullptr;
+            // weights are held as exp2(s + off) = 2^14 exp(score - max)
+            float off = INFINITY, l = 0.0f;
+            bool bad = false;
+            for (int u = c.u0; u < c.u1; ++u, ++g)
+            {
+                const uint32_t b = g & 1u;
+                if (!wait(smem_addr(&sm.s_full[b]), (g >> 1) & 1u))
+                {
+                    ok = false;
+                    break;
+                }
+                rt_fence_after();
+                const uint32_t ts = tmem + lanes + RT_T_S + b * 64u;
+                float s[64];
+                rt_ld32(ts, s);
+                rt_ld32(ts + 32, s + 32);
+                const RtUnitInfo& in = sm.info[g % RT_INFO];
+                const float f = fmaxf(qf * in.k_down, 1.17549435e-38f);
+                const uint64_t seen = live ? rt_seen<TREE>(u, in.valid, limit, mask, a.mask_words) : 0ull;
+                if ((in.kbad[0] | in.kbad[1]) != 0u &&
+                    (seen & ((uint64_t)in.kbad[0] | (uint64_t)in.kbad[1] << 32)) != 0ull)
+                    bad = true;
+                if (!__all_sync(0xffffffffu, seen == ~0ull))
+                {
+                    const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                    {
+                        s[j] = (s0 >> j) & 1u ? s[j] : -INFINITY;
+                        s[32 + j] = (s1 >> j) & 1u ? s[32 + j] : -INFINITY;
+                    }
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int j = 4; j < 64; ++j)
+                    mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float noff = fminf(off, 14.0f - top * f);
+                const float use = noff < INFINITY ? noff : 0.0f;
+                const float corr = rt_exp2(use - off); // 0 before the first key
+                off = noff;
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 f2 = make_float2(f, f), use2 = make_float2(use, use);
+#pragma unroll
+                for (int j0 = 0; j0 < 4; ++j0)
+                {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                    {
+                        float2 x = fma2_rn(make_float2(s[j0 * 16 + 2 * j], s[j0 * 16 + 2 * j + 1]), f2, use2);
+                        x.x = rt_exp2(x.x);
+                        x.y = rt_exp2(x.y);
+                        sum[j & 1] = rt_add2(sum[j & 1], x);
+                        rt_split2(x.x, x.y, hi[j], lo[j]);
+                    }
+                    rt_st8(ts + j0 * 8, hi);
+                    rt_st8(ts + 32 + j0 * 8, lo);
+                }
+                l = fmaf(l, corr, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                sm.alpha[g & 3u][i] = corr;
+                if (u + 1 == c.u1)
+                    sm.stats[item & 3u][i] = make_float2(bad ? __uint_as_float(0x7FC00000u) : l, off);
+                rt_wait_st();
+                rt_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(smem_addr(&sm.p_full[b]));
+            }
+        }
+    }
+    else if (warp < 12)
+    {
+        // ---- output sums: thread = row
+        rt_regs_inc<RT_REGS_O>();
+        const int i = (warp & 3) * 32 + lane, ti = i / G, gi = i - ti * G;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        uint32_t g = 0, item = 0;
+        bool ok = true;
+        RtCursor<TREE> c;
+        for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
+        {
+            const int r = c.t * R + ti;
+            const bool live = ti < R && r < c.q.n;
+            float acc[HDP];
+#pragma unroll
+            for (int d = 0; d < HDP; ++d)
+                acc[d] = 0.0f;
+            float2 stat = make_float2(0.0f, INFINITY);
+            bool bad = false;
+            for (int u = c.u0; u < c.u1; ++u, ++g)
+            {
+                const uint32_t b = g & 1u;
+                if (!wait(smem_addr(&sm.o_full[b]), (g >> 1) & 1u))
+                {
+                    ok = false;
+                    break;
+                }
+                rt_fence_after();
+                const float corr = sm.alpha[g & 3u][i];
+                const RtUnitInfo& in = sm.info[g % RT_INFO];
+                const float f = in.v_down;
+                if ((in.vbad[0] | in.vbad[1]) != 0u && live)
+                {
+                    const uint64_t seen = rt_seen<TREE>(
+                        u, in.valid, TREE ? c.q.past : min(c.q.past, INT_MAX - c.q.n) + r,
+                        TREE ? a.mask + (size_t)(c.q.begin + r) * a.mask_words : nullptr, a.mask_words);
+                    bad |= (seen & ((uint64_t)in.vbad[0] | (uint64_t)in.vbad[1] << 32)) != 0ull;
+                }
+                if (u + 1 == c.u1)
+                    stat = sm.stats[item & 3u][i];
+                const float2 c2 = make_float2(corr, corr), f2 = make_float2(f, f);
+#pragma unroll
+                for (int d0 = 0; d0 < HDP; d0 += 32)
+                {
+                    float t[32];
+                    rt_ld32(tmem + lanes + RT_T_O + b * 128u + d0, t);
+#pragma unroll
+                    for (int d = 0; d < 32; d += 2)
+                    {
+                        const float2 x = mul2_rn(make_float2(t[d], t[d + 1]), f2);
+                        const float2 y = fma2_rn(make_float2(acc[d0 + d], acc[d0 + d + 1]), c2, x);
+                        acc[d0 + d] = y.x;
+                        acc[d0 + d + 1] = y.y;
+                    }
+                }
+                rt_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(smem_addr(&sm.o_empty[b]));
+            }
+            if (!ok)
+                break;
+            const float l = bad ? __uint_as_float(0x7FC00000u) : stat.x;
+            if (c.whole)
+            {
+                if (live)
+                {
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    float4* o = reinterpret_cast<float4*>(a.out + (size_t)(c.q.begin + r) * a.ldo + (size_t)(c.h * G + gi) * hd);
+#pragma unroll
+                    for (int d = 0; d < HDP; d += 4)
+                        if (d < hd)
+                            o[d / 4] = make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+                }
+            }
+            else
+            {
+                float* slot = rt_slot<HDP>(a, blockIdx.x, item == 0 ? 0 : 1);
+                float4* o = reinterpret_cast<float4*>(slot + (size_t)i * HDP);
+#pragma unroll
+                for (int d = 0; d < HDP; d += 4)
+                    o[d / 4] = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+                reinterpret_cast<float2*>(slot + 128 * HDP)[i] = make_float2(l, stat.y);
+            }
+        }
+    }
+    else
+    {
+        // ---- a stage from fp32 to its fp16 parts, in place
+        rt_regs_dec<RT_REGS_CV>();
+        const int ct = tid - 12 * 32, cw = ct >> 5;
+        constexpr int NCH = 64 * HDP / 4 / RT_CONV_THREADS; // 16-byte pieces a thread
+        uint32_t pos = 0, g = 0;
+        auto convert = [&](uint32_t unit, bool is_k) -> bool {
+            const bool got = wait(bar_raw(pos), phase(pos));
+            const uint32_t stage = stage_at(pos), par = pos & 1u;
+            RtUnitInfo& in = sm.info[unit % RT_INFO];
+            const int valid = got ? sm.stage_valid[pos % NS] : 0;
+            float4 x[NCH];
+            uint32_t mb = 0;
+            auto bits = [](const float4& v) {
+                return max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu),
+                           max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
+            };
+#pragma unroll
+            for (int n = 0; n < NCH; ++n)
+            {
+                const int f = n * RT_CONV_THREADS + ct, row = f / (HDP / 4), c = f % (HDP / 4);
+                x[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (row < valid && c * 4 < hd)
+                {
+                    const uint4 w = lds128(stage + (uint32_t)(row * hd + c * 4) * 4u);
+                    x[n] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+                }
+                mb = max(mb, bits(x[n]));
+            }
+            if (mb >= 0x7F800000u)
+            {
+                // NaN or infinity: the key is noted and its values are zeros
+                mb = 0;
+#pragma unroll
+                for (int n = 0; n < NCH; ++n)
+                {
+                    if (bits(x[n]) >= 0x7F800000u)
+                    {
+                        const int row = (n * RT_CONV_THREADS + ct) / (HDP / 4);
+                        atomicOr(is_k ? &in.kbad[row >> 5] : &in.vbad[row >> 5], 1u << (row & 31));
+                        x[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                    mb = max(mb, bits(x[n]));
+                }
+            }
+            mb = __reduce_max_sync(0xffffffffu, mb);
+            if (lane == 0)
+                sm.wmax[par][cw] = mb;
+            // every read of the stage is done; a failed wait ends all eight warps together
+            if (named_bar_or(1, RT_CONV_THREADS, !got))
+                return false;
+#pragma unroll
+            for (int w = 0; w < RT_CONV_THREADS / 32; ++w)
+                mb = max(mb, sm.wmax[par][w]);
+            float up, down;
+            rt_scale_of(mb, up, down);
+            if (ct == 0)
+            {
+                if (is_k)
+                {
+                    in.k_down = down;
+                    in.valid = valid;
+                    // the unit after the next one's notes (its slot's last readers are long done)
+                    RtUnitInfo& later = sm.info[(unit + 2) % RT_INFO];
+                    later.kbad[0] = later.kbad[1] = later.vbad[0] = later.vbad[1] = 0u;
+                }
+                else
+                    in.v_down = down;
+            }
+#pragma unroll
+            for (int n = 0; n < NCH; ++n)
+            {
+                const int f = n * RT_CONV_THREADS + ct, row = f / (HDP / 4), c = f % (HDP / 4);
+                uint32_t h0, l0, h1, l1;
+                rt_split2(x[n].x * up, x[n].y * up, h0, l0);
+                rt_split2(x[n].z * up, x[n].w * up, h1, l1);
+                const int e = (c & 15) * 4; // element of the 64-dim block
+                const uint32_t at = stage + (uint32_t)(c >> 4) * 8192u + (uint32_t)row * 128u +
+                                    (uint32_t)(((e >> 3) ^ (row & 7)) * 16 + (e & 7) * 2);
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(h0), "r"(h1) : "memory");
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + NB * 8192u), "r"(l0), "r"(l1) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the MMA reads through the async proxy
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(bar_conv(pos));
+            ++pos;
+            return true;
+        };
+        bool ok = true;
+        RtCursor<TREE> c;
+        for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R))
+            for (int u = c.u0; u < c.u1 && ok; ++u, ++g)
+            {
+                if (u == c.u0 && g > 0)
+                    ok = convert(g - 1, false);
+                ok = ok && convert(g, true);
+                if (ok && u > c.u0)
+                    ok = convert(g - 1, false);
+            }
+        if (ok && g > 0)
+            convert(g - 1, false);
+    }
+    rt_fence_before();
+    __syncthreads();
+    if (warp == 1)
+    {
+        // every MMA issued is done before its tensor memory is given back
+        if (lane == 0)
+            mbar_wait_bounded(smem_addr(&sm.done), 0, RT_WAIT_LIMIT_NS);
+        __syncwarp();
+        rt_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(RT_T_COLS) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the partial sums of the tiles that a share's end went through: CTA
+// (boundary c, 8 rows), one row a warp. The tile's CTAs are taken in order.
+// ---------------------------------------------------------------------------
+constexpr int RJ_WARPS = 8;
+
+template <int HDP, bool TREE>
+__global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const AttnRowsArgs a, int grid)
+{
+    pdl_wait();
+    const int c0 = blockIdx.x + 1, lane = threadIdx.x & 31;
+    const RtStart* starts = reinterpret_cast<const RtStart*>(a.workspace);
+    const RtStart st = starts[c0];
+    // the share of CTA c0 starts inside a tile, and no earlier one does
+    if (st.u == 0 || st.begin >= st.total)
+        return;
+    const unsigned long long t0 = st.begin - (unsigned)st.u;
+    if (rt_share(st.total, c0 - 1, grid) > t0)
+        return;
+    const int G = a.n_heads / a.n_kv, R = 128 / G, i = blockIdx.y * RJ_WARPS + (threadIdx.x >> 5), ti = i / G;
+    const RtSeq q = rt_seq(a, st.s, R);
+    const int r = st.t * R + ti;
+    if (ti >= R || r >= q.n)
+        return;
+    const unsigned long long t1 = t0 + (unsigned)((rt_keys(q, TREE, R, st.t) + 63) / 64);
+    // the first share with a unit of the tile: the last one that starts at or before it and is not empty
+    int first = c0 - 1;
+    while (first > 0 && rt_share(st.total, first, grid) > t0)
+        --first;
+    while (rt_share(st.total, first + 1, grid) <= t0)
+        ++first;
+    float off = INFINITY;
+    for (int pass = 0; pass < 2; ++pass)
+    {
+        float l = 0.0f, acc[HDP / 32];
+#pragma unroll
+        for (int d = 0; d < HDP / 32; ++d)
+            acc[d] = 0.0f;
+        for (int c = first; c < grid; ++c)
+        {
+            const unsigned long long b = rt_share(st.total, c, grid);
+            if (b >= t1)
+                break;
+            if (rt_share(st.total, c + 1, grid) == b)
+                continue;
+            const float* slot = rt_slot<HDP>(a, c, b >= t0 ? 0 : 1);
+            const float2 s = __ldcg(reinterpret_cast<const float2*>(slot + 128 * HDP) + i);
+            if (pass == 0)
+                off = fminf(off, s.y);
+            else
+            {
+                const float w = s.y < INFINITY ? rt_exp2(off - s.y) : 0.0f;
+                l = fmaf(s.x, w, l);
+#pragma unroll
+                for (int d = 0; d < HDP / 32; ++d)
+                    acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), w, acc[d]);
+            }
+        }
+        if (pass == 1)
+        {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            float* o = a.out + (size_t)(q.begin + r) * a.ldo + (size_t)(st.h * G + (i - ti * G)) * a.head_dim;
+#pragma unroll
+            for (int d = 0; d < HDP / 32; ++d)
+                if (d * 32 + lane < a.head_dim)
+                    o[d * 32 + lane] = acc[d] * inv;
+        }
+    }
+}
+
+} // namespace aaedn_dev
