@@ -47,17 +47,18 @@
 namespace aaedn_dev
 {
 
-constexpr int RT_WARPS = 20, RT_THREADS = RT_WARPS * 32;
+constexpr int RT_WARPS = 24, RT_THREADS = RT_WARPS * 32;
 constexpr int RT_CONV_THREADS = 256;
-constexpr int RT_REGS = 96; // registers a thread at launch: 65536 / 640, whole eights
+constexpr int RT_REGS = 80; // registers a thread at launch: 65536 / 768, whole eights
 // the warpgroups' shares after setmaxnreg: together the launch's
-constexpr int RT_REGS_IO = 48, RT_REGS_SM = 120, RT_REGS_O = 184, RT_REGS_CV = 64;
-static_assert(RT_REGS_IO + RT_REGS_SM + RT_REGS_O + 2 * RT_REGS_CV == 5 * RT_REGS, "register shares");
+constexpr int RT_REGS_IO = 40, RT_REGS_SM = 112, RT_REGS_O = 168, RT_REGS_CV = 56, RT_REGS_Q = 48;
+static_assert(RT_REGS_IO + RT_REGS_SM + RT_REGS_O + 2 * RT_REGS_CV + RT_REGS_Q == 6 * RT_REGS, "register shares");
 constexpr uint64_t RT_WAIT_LIMIT_NS = 2000000000ull;
 constexpr int RT_INFO = 16; // units whose scales are kept
 
-// tensor memory columns
-constexpr uint32_t RT_T_S = 0, RT_T_O = 128, RT_T_Q = 384, RT_T_QLO = 64, RT_T_COLS = 512;
+// tensor memory columns (the CTA allocates all of it, so its base is 0): S and
+// P of two units, O of one, Q of two tiles (high parts, then low parts)
+constexpr uint32_t RT_T_S = 0, RT_T_O = 128, RT_T_Q = 256, RT_T_QLO = 64, RT_T_COLS = 512;
 
 template <int HDP> // head_dim rounded up to whole 64
 struct RtCfg
@@ -293,22 +294,52 @@ __device__ __forceinline__ void rt_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void rt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void rt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of the warp's 32 lanes; the registers hold them after the wait.
-__device__ __forceinline__ void rt_ld32(uint32_t taddr, float* v)
+// N columns of the warp's 32 lanes; one statement, so that the registers are
+// read only after the wait.
+template <int N>
+__device__ __forceinline__ void rt_ld(uint32_t taddr, float* v);
+
+template <>
+__device__ __forceinline__ void rt_ld<16>(uint32_t taddr, float* v)
 {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+                 "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15 "
+                 "}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 16; ++i)
+        v[i] = __uint_as_float(r[i]);
+}
+
+template <>
+__device__ __forceinline__ void rt_ld<64>(uint32_t taddr, float* v)
+{
+    uint32_t r[64];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+                 "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+                 "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
+                 "}, [%64];\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, "
+                 "%52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+                 "}, [%65];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+                   "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+                   "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+                   "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+                   "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr), "r"(taddr + 32u)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i)
         v[i] = __uint_as_float(r[i]);
 }
 
@@ -319,13 +350,24 @@ __device__ __forceinline__ void rt_st8(uint32_t taddr, const uint32_t (&r)[8])
                  : "memory");
 }
 
-// D[tensor memory] (+)= A[tensor memory] B[shared memory], fp16 in, fp32 out
-__device__ __forceinline__ void rt_mma(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc)
+// D[tensor memory] (+)= A[tensor memory] B[shared memory], fp16 in, fp32 out.
+// The descriptor comes as its two words: steps along the operand only add to
+// the low one.
+__device__ __forceinline__ void rt_mma(uint32_t d, uint32_t a, uint32_t desc_lo, uint32_t desc_hi, uint32_t idesc,
+                                       uint32_t acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                 "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 desc;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 desc, {%2, %3};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], desc, %4, p;\n\t}" ::"r"(d),
+                 "r"(a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(acc)
                  : "memory");
+}
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool rt_elect()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 __device__ __forceinline__ void rt_commit(uint32_t mbar)
@@ -337,10 +379,10 @@ __device__ __forceinline__ void rt_commit(uint32_t mbar)
 // K-major, 8-key groups 1024 bytes apart. V: the same bytes as an MN-major
 // operand: 64-dim blocks 8192 bytes apart (leading offset), 8-key groups
 // 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t rt_desc(uint32_t saddr, uint32_t lead)
+constexpr uint32_t RT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29); // stride 1024, version 1, 128-byte swizzle
+__device__ __forceinline__ uint32_t rt_desc_lo(uint32_t saddr, uint32_t lead)
 {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
-           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+    return ((saddr >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
 }
 // kind::f16 with fp16 A and B, fp32 D, M = 128; b_mn: B is MN-major
 __host__ __device__ constexpr uint32_t rt_idesc(int n, bool b_mn)
@@ -376,6 +418,17 @@ __device__ __forceinline__ void rt_split2(float x, float y, uint32_t& hi, uint32
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// max(m, |x|, |y|, |z|, |w|); a NaN stays
+__device__ __forceinline__ float rt_max_abs(float m, const float4& v)
+{
+    float a = m;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.x)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.y)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.z)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.w)));
+    return a;
+}
+
 // The power of two that puts a magnitude with these bits at 2^14..2^15, and
 // its inverse (both normal numbers).
 __device__ __forceinline__ void rt_scale_of(uint32_t max_bits, float& up, float& down)
@@ -407,13 +460,14 @@ struct RtUnitInfo
 struct RtShared
 {
     uint64_t raw[8], conv[8], free_[8]; // per stage: copied, converted, read by the MMAs
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
+    uint64_t s_full[2], p_full[2], o_full, o_empty, q_full[2], q_empty[2], done;
     uint32_t tmem, abort;
     RtStart start;
     int stage_valid[8];
     uint32_t wmax[2][8];
     RtUnitInfo info[RT_INFO];
     float alpha[4][128];
+    float q_down[4][128]; // what undoes an item's rows' scaling of Q
     float2 stats[4][128]; // (sum, offset) of an item's rows
 };
 
@@ -510,10 +564,11 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             {
                 mbar_init(smem_addr(&sm.s_full[i]), 1);
                 mbar_init(smem_addr(&sm.p_full[i]), 4);
-                mbar_init(smem_addr(&sm.o_full[i]), 1);
-                mbar_init(smem_addr(&sm.o_empty[i]), 4);
+                mbar_init(smem_addr(&sm.q_full[i]), 4);
+                mbar_init(smem_addr(&sm.q_empty[i]), 1);
             }
-            mbar_init(smem_addr(&sm.q_full), 4);
+            mbar_init(smem_addr(&sm.o_full), 1);
+            mbar_init(smem_addr(&sm.o_empty), 4);
             mbar_init(smem_addr(&sm.done), 1);
             mbar_init_fence();
             sm.abort = 0u;
@@ -532,9 +587,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
     rt_fence_before();
     __syncthreads();
     rt_fence_after();
-    const uint32_t tmem = sm.tmem;
+    constexpr uint32_t tmem = 0u; // all columns are the CTA's
     const RtStart st0 = sm.start;
-    const unsigned long long share = rt_share(st0.total, blockIdx.x + 1, gridDim.x) - st0.begin;
+    unsigned long long share = rt_share(st0.total, blockIdx.x + 1, gridDim.x) - st0.begin;
+    if (sm.tmem != tmem) // cannot be: nothing runs on other columns
+    {
+        share = 0;
+        fail();
+    }
+    // wait() for a whole warp: its lanes go on, or give up, together
+    auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
 
     if (warp < 4)
     {
@@ -568,28 +630,22 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R))
             {
                 const int* pt = rows_page_table(a, c.s);
-                for (int u0 = c.u0; u0 < c.u1 && ok; u0 += 32)
+                int mine = 0;
+                for (int u = c.u0; u < c.u1 && ok; ++u)
                 {
-                    const int mine = u0 + lane < c.u1 ? __ldg(pt + u0 + lane) : 0;
-                    for (int u = u0; u < min(u0 + 32, c.u1) && ok; ++u)
-                    {
-                        const int page = __shfl_sync(0xffffffffu, mine, u - u0);
-                        const int valid = min(64, c.keys - u * 64);
-                        if (lane == 0)
-                        {
-                            if (u == c.u0 && due)
-                                ok = emit(a.v, vpage, vh, vvalid);
-                            if (ok)
-                                ok = emit(a.k, page, c.h, valid);
-                            if (ok && u > c.u0)
-                                ok = emit(a.v, vpage, vh, vvalid);
-                        }
-                        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                        vpage = page;
-                        vh = c.h;
-                        vvalid = valid;
-                        due = true;
-                    }
+                    const int k = (u - c.u0) & 31;
+                    if (k == 0) // the next 32 page numbers, one a lane
+                        mine = u + lane < c.u1 ? __ldg(pt + u + lane) : 0;
+                    const int page = __shfl_sync(0xffffffffu, mine, k), valid = min(64, c.keys - u * 64);
+                    if (lane == 0)
+                        for (int v = 0; v < 2 && ok; ++v) // K of this unit, V of the one before
+                            if (v == 0 || due)
+                                ok = emit(v ? a.v : a.k, v ? vpage : page, v ? vh : c.h, v ? vvalid : valid);
+                    ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                    vpage = page;
+                    vh = c.h;
+                    vvalid = valid;
+                    due = true;
                 }
             }
             if (lane == 0)
@@ -604,64 +660,77 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
         }
         else if (warp == 1)
         {
-            // ---- MMA issuer (one thread)
-            if (lane == 0)
+            // ---- MMA issuer: the warp walks the units, one lane issues
+            constexpr uint32_t id_qk = rt_idesc(64, false), id_pv = rt_idesc(HDP, true);
+            constexpr uint32_t QLO = HDP == 128 ? RT_T_QLO : 32u;
+            uint32_t pos = 0, g = 0, item = 0;
+            RtCursor<TREE> c;
+            bool more = c.start(a, st0, share, R), ok = true;
+            int u = more ? c.u0 : 0;
+            while (ok)
             {
-                constexpr uint32_t id_qk = rt_idesc(64, false), id_pv = rt_idesc(HDP, true);
-                uint32_t pos = 0, g = 0, item = 0;
-                bool ok = true;
-                auto qk = [&](bool first) {
-                    if (first && !wait(smem_addr(&sm.q_full), item & 1u))
-                        return false;
-                    if (!wait(bar_conv(pos), phase(pos)))
-                        return false;
+                if (more)
+                {
+                    const uint32_t qb = item & 1u;
+                    if ((u == c.u0 && !wait_all(smem_addr(&sm.q_full[qb]), (item >> 1) & 1u)) || !wait_all(bar_conv(pos), phase(pos)))
+                        break;
                     rt_fence_after();
-                    const uint32_t d = tmem + RT_T_S + (g & 1u) * 64u, kb = stage_at(pos);
-                    const uint32_t qh = tmem + RT_T_Q, ql = qh + (HDP == 128 ? RT_T_QLO : 32u);
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) // q_hi k_lo, q_lo k_hi, q_hi k_hi
-#pragma unroll
-                        for (int k = 0; k < HDP / 16; ++k)
-                            rt_mma(d, (p == 1 ? ql : qh) + k * 8,
-                                   rt_desc(kb + (p == 0 ? NB * 8192u : 0u) + (k >> 2) * 8192u + (k & 3) * 32u, 16u), id_qk,
-                                   (p | k) != 0 ? 1u : 0u);
-                    rt_commit(smem_addr(&sm.s_full[g & 1u]));
-                    rt_commit(bar_free(pos));
-                    ++pos;
-                    return true;
-                };
-                auto pv = [&](uint32_t j) { // unit j
-                    if (!wait(bar_conv(pos), phase(pos)) || !wait(smem_addr(&sm.p_full[j & 1u]), (j >> 1) & 1u) ||
-                        (j >= 2 && !wait(smem_addr(&sm.o_empty[j & 1u]), ((j >> 1) & 1u) ^ 1u)))
-                        return false;
-                    rt_fence_after();
-                    const uint32_t d = tmem + RT_T_O + (j & 1u) * 128u, vb = stage_at(pos);
-                    const uint32_t ph = tmem + RT_T_S + (j & 1u) * 64u, pl = ph + 32u;
-#pragma unroll
-                    for (int p = 0; p < 3; ++p)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            rt_mma(d, (p == 1 ? pl : ph) + k * 8,
-                                   rt_desc(vb + (p == 0 ? NB * 8192u : 0u) + k * 2048u, 8192u), id_pv, (p | k) != 0 ? 1u : 0u);
-                    rt_commit(smem_addr(&sm.o_full[j & 1u]));
-                    rt_commit(bar_free(pos));
-                    ++pos;
-                    return true;
-                };
-                RtCursor<TREE> c;
-                for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
-                    for (int u = c.u0; u < c.u1 && ok; ++u, ++g)
+                    const uint32_t k_hi = rt_desc_lo(stage_at(pos), 16u), d = RT_T_S + (g & 1u) * 64u;
+                    const bool last = u + 1 == c.u1;
+                    if (rt_elect())
                     {
-                        if (u == c.u0 && g > 0)
-                            ok = pv(g - 1);
-                        ok = ok && qk(u == c.u0);
-                        if (ok && u > c.u0)
-                            ok = pv(g - 1);
+#pragma unroll 1
+                        for (uint32_t p = 0; p < 3; ++p) // q_hi k_lo, q_lo k_hi, q_hi k_hi
+                        {
+                            const uint32_t q = RT_T_Q + qb * 128u + (p == 1 ? QLO : 0u), k = k_hi + (p == 0 ? NB * 512u : 0u);
+#pragma unroll
+                            for (uint32_t n = 0; n < HDP / 16; ++n)
+                                rt_mma(d, q + n * 8u, k + (n >> 2) * 512u + (n & 3u) * 2u, RT_DESC_HI, id_qk, p | n);
+                        }
+                        rt_commit(smem_addr(&sm.s_full[g & 1u]));
+                        rt_commit(bar_free(pos));
+                        if (last)
+                            rt_commit(smem_addr(&sm.q_empty[qb]));
                     }
-                if (ok && g > 0)
-                    pv(g - 1);
-                rt_commit(smem_addr(&sm.done)); // every MMA issued, whatever happened
+                    __syncwarp();
+                    ++pos;
+                }
+                if (g > 0) // P V of the unit before
+                {
+                    const uint32_t j = g - 1u;
+                    if (!wait_all(bar_conv(pos), phase(pos)) || !wait_all(smem_addr(&sm.p_full[j & 1u]), (j >> 1) & 1u) ||
+                        (j >= 1u && !wait_all(smem_addr(&sm.o_empty), (j - 1u) & 1u)))
+                        break;
+                    rt_fence_after();
+                    const uint32_t v_hi = rt_desc_lo(stage_at(pos), 8192u), ph = RT_T_S + (j & 1u) * 64u;
+                    if (rt_elect())
+                    {
+#pragma unroll 1
+                        for (uint32_t p = 0; p < 3; ++p) // p_hi v_lo, p_lo v_hi, p_hi v_hi
+                        {
+                            const uint32_t w = ph + (p == 1 ? 32u : 0u), v = v_hi + (p == 0 ? NB * 512u : 0u);
+#pragma unroll
+                            for (uint32_t n = 0; n < 4; ++n)
+                                rt_mma(RT_T_O, w + n * 8u, v + n * 128u, RT_DESC_HI, id_pv, p | n);
+                        }
+                        rt_commit(smem_addr(&sm.o_full));
+                        rt_commit(bar_free(pos));
+                    }
+                    __syncwarp();
+                    ++pos;
+                }
+                if (!more)
+                    break;
+                ++g;
+                if (++u >= c.u1)
+                {
+                    more = c.next(a, R);
+                    u = c.u0;
+                    ++item;
+                }
             }
+            if (rt_elect())
+                rt_commit(smem_addr(&sm.done)); // every MMA issued, whatever happened
             __syncwarp();
         }
     }
@@ -669,54 +738,18 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
     {
         // ---- softmax: thread = row
         rt_regs_inc<RT_REGS_SM>();
-        const int i = (warp & 3) * 32 + lane, ti = i / G, gi = i - ti * G;
+        const int i = (warp & 3) * 32 + lane, ti = i / G;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         constexpr float LOG2E = 1.4426950408889634f;
-        const float qs = fabsf(a.scale) * LOG2E, sign = a.scale < 0.0f ? -1.0f : 1.0f;
+        const float qs = fabsf(a.scale) * LOG2E;
         uint32_t g = 0, item = 0;
         bool ok = true;
         RtCursor<TREE> c;
         for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
         {
-            // the row's query into tensor memory (every product with the last
-            // item's is done: its last S was waited for)
             const int r = c.t * R + ti;
             const bool live = ti < R && r < c.q.n;
-            const float4* qr = reinterpret_cast<const float4*>(a.q + (size_t)(c.q.begin + (live ? r : 0)) * a.ldq +
-                                                               (size_t)(c.h * G + gi) * hd);
-            uint32_t mb = 0;
-            if (live)
-#pragma unroll 8
-                for (int d = 0; d < HDP / 4; ++d)
-                    if (d * 4 < hd)
-                    {
-                        const float4 x = qr[d];
-                        mb = max(max(mb, max(__float_as_uint(x.x) & 0x7FFFFFFFu, __float_as_uint(x.y) & 0x7FFFFFFFu)),
-                                 max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu));
-                    }
-            float q_up, q_down;
-            rt_scale_of(mb, q_up, q_down);
-            q_up *= sign;
-#pragma unroll
-            for (int d0 = 0; d0 < HDP / 16; ++d0)
-            {
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                {
-                    const float4 x = live && (d0 * 4 + d) * 4 < hd ? qr[d0 * 4 + d] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    rt_split2(x.x * q_up, x.y * q_up, hi[2 * d], lo[2 * d]);
-                    rt_split2(x.z * q_up, x.w * q_up, hi[2 * d + 1], lo[2 * d + 1]);
-                }
-                rt_st8(tmem + lanes + RT_T_Q + d0 * 8, hi);
-                rt_st8(tmem + lanes + RT_T_Q + (HDP == 128 ? RT_T_QLO : 32u) + d0 * 8, lo);
-            }
-            rt_wait_st();
-            rt_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(smem_addr(&sm.q_full));
-            const float qf = qs * q_down;
+            float qf = 0.0f;
             const int limit = TREE ? c.q.past : min(c.q.past, INT_MAX - c.q.n) + r; // past + r: far behind cap when clamped
             const uint64_t* mask = TREE ? a.mask + (size_t)(c.q.begin + (live ? r : 0)) * a.mask_words : nullptr;
             // weights are held as exp2(s + off) = 2^14 exp(score - max)
@@ -725,16 +758,17 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             for (int u = c.u0; u < c.u1; ++u, ++g)
             {
                 const uint32_t b = g & 1u;
-                if (!wait(smem_addr(&sm.s_full[b]), (g >> 1) & 1u))
+                if (!wait_all(smem_addr(&sm.s_full[b]), (g >> 1) & 1u))
                 {
                     ok = false;
                     break;
                 }
                 rt_fence_after();
                 const uint32_t ts = tmem + lanes + RT_T_S + b * 64u;
+                if (u == c.u0)
+                    qf = qs * sm.q_down[item & 3u][i];
                 float s[64];
-                rt_ld32(ts, s);
-                rt_ld32(ts + 32, s + 32);
+                rt_ld<64>(ts, s);
                 const RtUnitInfo& in = sm.info[g % RT_INFO];
                 const float f = fmaxf(qf * in.k_down, 1.17549435e-38f);
                 const uint64_t seen = live ? rt_seen<TREE>(u, in.valid, limit, mask, a.mask_words) : 0ull;
@@ -811,8 +845,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             bool bad = false;
             for (int u = c.u0; u < c.u1; ++u, ++g)
             {
-                const uint32_t b = g & 1u;
-                if (!wait(smem_addr(&sm.o_full[b]), (g >> 1) & 1u))
+                if (!wait_all(smem_addr(&sm.o_full), g & 1u))
                 {
                     ok = false;
                     break;
@@ -832,12 +865,12 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     stat = sm.stats[item & 3u][i];
                 const float2 c2 = make_float2(corr, corr), f2 = make_float2(f, f);
 #pragma unroll
-                for (int d0 = 0; d0 < HDP; d0 += 32)
+                for (int d0 = 0; d0 < HDP; d0 += 16)
                 {
-                    float t[32];
-                    rt_ld32(tmem + lanes + RT_T_O + b * 128u + d0, t);
+                    float t[16];
+                    rt_ld<16>(tmem + lanes + RT_T_O + d0, t);
 #pragma unroll
-                    for (int d = 0; d < 32; d += 2)
+                    for (int d = 0; d < 16; d += 2)
                     {
                         const float2 x = mul2_rn(make_float2(t[d], t[d + 1]), f2);
                         const float2 y = fma2_rn(make_float2(acc[d0 + d], acc[d0 + d + 1]), c2, x);
@@ -848,7 +881,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 rt_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive(smem_addr(&sm.o_empty[b]));
+                    mbar_arrive(smem_addr(&sm.o_empty));
             }
             if (!ok)
                 break;
@@ -876,24 +909,20 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             }
         }
     }
-    else
+    else if (warp < 20)
     {
         // ---- a stage from fp32 to its fp16 parts, in place
         rt_regs_dec<RT_REGS_CV>();
         const int ct = tid - 12 * 32, cw = ct >> 5;
         constexpr int NCH = 64 * HDP / 4 / RT_CONV_THREADS; // 16-byte pieces a thread
-        uint32_t pos = 0, g = 0;
+        uint32_t pos = 0;
         auto convert = [&](uint32_t unit, bool is_k) -> bool {
             const bool got = wait(bar_raw(pos), phase(pos));
             const uint32_t stage = stage_at(pos), par = pos & 1u;
             RtUnitInfo& in = sm.info[unit % RT_INFO];
             const int valid = got ? sm.stage_valid[pos % NS] : 0;
             float4 x[NCH];
-            uint32_t mb = 0;
-            auto bits = [](const float4& v) {
-                return max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu),
-                           max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
-            };
+            float mx = 0.0f; // NaN is kept
 #pragma unroll
             for (int n = 0; n < NCH; ++n)
             {
@@ -904,25 +933,25 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     const uint4 w = lds128(stage + (uint32_t)(row * hd + c * 4) * 4u);
                     x[n] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
                 }
-                mb = max(mb, bits(x[n]));
+                mx = rt_max_abs(mx, x[n]);
             }
-            if (mb >= 0x7F800000u)
+            if (!(mx < INFINITY))
             {
                 // NaN or infinity: the key is noted and its values are zeros
-                mb = 0;
+                mx = 0.0f;
 #pragma unroll
                 for (int n = 0; n < NCH; ++n)
                 {
-                    if (bits(x[n]) >= 0x7F800000u)
+                    if (!(rt_max_abs(0.0f, x[n]) < INFINITY))
                     {
                         const int row = (n * RT_CONV_THREADS + ct) / (HDP / 4);
                         atomicOr(is_k ? &in.kbad[row >> 5] : &in.vbad[row >> 5], 1u << (row & 31));
                         x[n] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
-                    mb = max(mb, bits(x[n]));
+                    mx = rt_max_abs(mx, x[n]);
                 }
             }
-            mb = __reduce_max_sync(0xffffffffu, mb);
+            uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)); // not negative: ordered as integers
             if (lane == 0)
                 sm.wmax[par][cw] = mb;
             // every read of the stage is done; a failed wait ends all eight warps together
@@ -966,19 +995,68 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             ++pos;
             return true;
         };
+        // K of every unit, each followed by V of the unit before; the last V
+        const uint32_t left = (uint32_t)share;
+        bool ok = true;
+        for (uint32_t e = 1; e <= 2u * left && ok; ++e)
+        {
+            // e: 1 K0, 2 K1, 3 V0, 4 K2, 5 V1, ... 2 left: the last V
+            const bool is_k = e == 1u || (!(e & 1u) && e < 2u * left);
+            ok = convert(is_k ? e >> 1 : (e == 2u * left ? left - 1u : (e - 3u) >> 1), is_k);
+        }
+    }
+    else
+    {
+        // ---- the next tile's queries into tensor memory: thread = row
+        rt_regs_dec<RT_REGS_Q>();
+        const int i = (warp & 3) * 32 + lane, ti = i / G, gi = i - ti * G;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f; // the softmax takes |scale|
+        uint32_t item = 0;
         bool ok = true;
         RtCursor<TREE> c;
-        for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R))
-            for (int u = c.u0; u < c.u1 && ok; ++u, ++g)
+        for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
+        {
+            const uint32_t qb = item & 1u;
+            const int r = c.t * R + ti;
+            const bool live = ti < R && r < c.q.n;
+            const float4* qr = reinterpret_cast<const float4*>(a.q + (size_t)(c.q.begin + (live ? r : 0)) * a.ldq +
+                                                               (size_t)(c.h * G + gi) * hd);
+            float mx = 0.0f; // NaN is kept
+            if (live)
+#pragma unroll 4
+                for (int d = 0; d < hd / 4; ++d)
+                    mx = rt_max_abs(mx, qr[d]);
+            float q_up, q_down;
+            rt_scale_of(__float_as_uint(mx) & 0x7FFFFFFFu, q_up, q_down);
+            q_up *= sign;
+            if (item >= 2 && !wait_all(smem_addr(&sm.q_empty[qb]), ((item >> 1) & 1u) ^ 1u))
             {
-                if (u == c.u0 && g > 0)
-                    ok = convert(g - 1, false);
-                ok = ok && convert(g, true);
-                if (ok && u > c.u0)
-                    ok = convert(g - 1, false);
+                ok = false;
+                break;
             }
-        if (ok && g > 0)
-            convert(g - 1, false);
+            rt_fence_after();
+            sm.q_down[item & 3u][i] = q_down;
+#pragma unroll 1
+            for (int d0 = 0; d0 < HDP / 16; ++d0)
+            {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                {
+                    const float4 x = live && (d0 * 4 + d) * 4 < hd ? qr[d0 * 4 + d] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    rt_split2(x.x * q_up, x.y * q_up, hi[2 * d], lo[2 * d]);
+                    rt_split2(x.z * q_up, x.w * q_up, hi[2 * d + 1], lo[2 * d + 1]);
+                }
+                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + d0 * 8, hi);
+                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + (HDP == 128 ? RT_T_QLO : 32u) + d0 * 8, lo);
+            }
+            rt_wait_st();
+            rt_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(smem_addr(&sm.q_full[qb]));
+        }
     }
     rt_fence_before();
     __syncthreads();
@@ -1024,43 +1102,60 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         --first;
     while (rt_share(st.total, first + 1, grid) <= t0)
         ++first;
-    float off = INFINITY;
-    for (int pass = 0; pass < 2; ++pass)
+    // lane j takes the weights of share first + j, 32 at a time
+    const float2 none = make_float2(0.0f, INFINITY);
+    auto stat_of = [&](int c) -> float2 {
+        if (c >= grid)
+            return none;
+        const unsigned long long b = rt_share(st.total, c, grid);
+        if (b >= t1 || rt_share(st.total, c + 1, grid) == b)
+            return none;
+        return __ldcg(reinterpret_cast<const float2*>(rt_slot<HDP>(a, c, b >= t0 ? 0 : 1) + 128 * HDP) + i);
+    };
+    int last = first; // the last share with a unit of the tile
     {
-        float l = 0.0f, acc[HDP / 32];
-#pragma unroll
-        for (int d = 0; d < HDP / 32; ++d)
-            acc[d] = 0.0f;
-        for (int c = first; c < grid; ++c)
+        int hi = grid - 1;
+        while (last < hi)
         {
-            const unsigned long long b = rt_share(st.total, c, grid);
-            if (b >= t1)
-                break;
-            if (rt_share(st.total, c + 1, grid) == b)
-                continue;
-            const float* slot = rt_slot<HDP>(a, c, b >= t0 ? 0 : 1);
-            const float2 s = __ldcg(reinterpret_cast<const float2*>(slot + 128 * HDP) + i);
-            if (pass == 0)
-                off = fminf(off, s.y);
+            const int mid = (last + hi + 1) >> 1;
+            if (rt_share(st.total, mid, grid) < t1)
+                last = mid;
             else
-            {
-                const float w = s.y < INFINITY ? rt_exp2(off - s.y) : 0.0f;
-                l = fmaf(s.x, w, l);
-#pragma unroll
-                for (int d = 0; d < HDP / 32; ++d)
-                    acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), w, acc[d]);
-            }
-        }
-        if (pass == 1)
-        {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            float* o = a.out + (size_t)(q.begin + r) * a.ldo + (size_t)(st.h * G + (i - ti * G)) * a.head_dim;
-#pragma unroll
-            for (int d = 0; d < HDP / 32; ++d)
-                if (d * 32 + lane < a.head_dim)
-                    o[d * 32 + lane] = acc[d] * inv;
+                hi = mid - 1;
         }
     }
+    float off = INFINITY;
+    for (int c = first; c <= last; c += 32)
+        off = fminf(off, -warp_max(-stat_of(c + lane).y));
+    float l = 0.0f, acc[HDP / 32];
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+        acc[d] = 0.0f;
+    for (int c = first; c <= last; c += 32)
+    {
+        const float2 s = stat_of(c + lane);
+        const float w = s.y < INFINITY ? rt_exp2(off - s.y) : 0.0f;
+        l += warp_sum(s.x * w);
+        const int n = min(32, last + 1 - c);
+#pragma unroll 4
+        for (int j = 0; j < n; ++j)
+        {
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            // an empty share (weight 0) has no sums: its slot is not read
+            const float* slot = rt_slot<HDP>(a, c + j, j > 0 || c > first || rt_share(st.total, first, grid) >= t0 ? 0 : 1);
+            const bool some = __shfl_sync(0xffffffffu, s.y, j) < INFINITY;
+#pragma unroll
+            for (int d = 0; d < HDP / 32; ++d)
+                if (some)
+                    acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), wj, acc[d]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float* o = a.out + (size_t)(q.begin + r) * a.ldo + (size_t)(st.h * G + (i - ti * G)) * a.head_dim;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+        if (d * 32 + lane < a.head_dim)
+            o[d * 32 + lane] = acc[d] * inv;
 }
 
 } // namespace aaedn_dev
