@@ -47,12 +47,13 @@
 namespace aaedn_dev
 {
 
-constexpr int RT_WARPS = 24, RT_THREADS = RT_WARPS * 32;
+constexpr int RT_WARPS = 28, RT_THREADS = RT_WARPS * 32;
+constexpr int RT_W_SM = 4, RT_W_O = 8, RT_W_CV = 16, RT_W_Q = 24; // first warps of the roles
 constexpr int RT_CONV_THREADS = 256;
-constexpr int RT_REGS = 80; // registers a thread at launch: 65536 / 768, whole eights
+constexpr int RT_REGS = 72; // registers a thread at launch: 65536 / 896, whole eights
 // the warpgroups' shares after setmaxnreg: together the launch's
-constexpr int RT_REGS_IO = 40, RT_REGS_SM = 112, RT_REGS_O = 168, RT_REGS_CV = 56, RT_REGS_Q = 48;
-static_assert(RT_REGS_IO + RT_REGS_SM + RT_REGS_O + 2 * RT_REGS_CV + RT_REGS_Q == 6 * RT_REGS, "register shares");
+constexpr int RT_REGS_IO = 40, RT_REGS_SM = 80, RT_REGS_O = 104, RT_REGS_CV = 64, RT_REGS_Q = 48;
+static_assert(RT_REGS_IO + RT_REGS_SM + 2 * RT_REGS_O + 2 * RT_REGS_CV + RT_REGS_Q == 7 * RT_REGS, "register shares");
 constexpr uint64_t RT_WAIT_LIMIT_NS = 2000000000ull;
 constexpr int RT_INFO = 16; // units whose scales are kept
 
@@ -63,10 +64,11 @@ constexpr uint32_t RT_T_S = 0, RT_T_O = 128, RT_T_Q = 256, RT_T_QLO = 64, RT_T_C
 template <int HDP> // head_dim rounded up to whole 64
 struct RtCfg
 {
-    static constexpr int NS = HDP == 128 ? 6 : 8; // stages of one page of K or V
+    static constexpr int NS = HDP == 128 ? 4 : 8; // stages of one page of K or V
     static constexpr uint32_t STAGE = 64u * HDP * 4u;
     static constexpr int NB = HDP / 64;
-    static constexpr size_t SMEM = (size_t)NS * STAGE + 1024; // + alignment slack
+    static constexpr uint32_t Q_ROW = HDP * 4u + 16u; // a query row in shared memory: no bank conflicts across rows
+    static constexpr size_t SMEM = (size_t)NS * STAGE + 128 * Q_ROW + 1024; // + alignment slack
 };
 
 // ---- the split of the work ----------------------------------------------------
@@ -112,8 +114,9 @@ __host__ __device__ inline int rt_keys(const RtSeq& q, bool tree, int R, int til
     return k < q.cap ? (int)k : q.cap;
 }
 
-// units of the first `tiles` tiles of one K/V head
-__host__ __device__ inline unsigned long long rt_units_before(const RtSeq& q, bool tree, int R, int tiles)
+// units of the first `tiles` tiles of one K/V head (a call: its code is used
+// once per CTA and would crowd the loops out of the instruction cache)
+__host__ __device__ __noinline__ unsigned long long rt_units_before(const RtSeq q, bool tree, int R, int tiles)
 {
     if (tiles <= 0)
         return 0;
@@ -176,7 +179,7 @@ __device__ __forceinline__ unsigned long long rt_share(unsigned long long total,
 
 // The position of unit `at` (one warp; the result in every lane).
 template <bool TREE>
-__device__ RtStart rt_locate(const AttnRowsArgs& a, int R, int cta, int grid)
+__device__ __noinline__ RtStart rt_locate(const AttnRowsArgs a, int R, int cta, int grid)
 {
     const int lane = threadIdx.x & 31;
     auto units_of = [&](int s) -> unsigned long long {
@@ -316,33 +319,6 @@ __device__ __forceinline__ void rt_ld<16>(uint32_t taddr, float* v)
         v[i] = __uint_as_float(r[i]);
 }
 
-template <>
-__device__ __forceinline__ void rt_ld<64>(uint32_t taddr, float* v)
-{
-    uint32_t r[64];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-                 "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-                 "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
-                 "}, [%64];\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, "
-                 "%52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
-                 "}, [%65];\n\ttcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
-                   "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
-                   "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
-                   "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-                   "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-                 : "r"(taddr), "r"(taddr + 32u)
-                 : "memory");
-#pragma unroll
-    for (int i = 0; i < 64; ++i)
-        v[i] = __uint_as_float(r[i]);
-}
-
 __device__ __forceinline__ void rt_st8(uint32_t taddr, const uint32_t (&r)[8])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
@@ -407,26 +383,37 @@ __device__ __forceinline__ float2 rt_add2(float2 a, float2 b)
     return d;
 }
 
-// x and y as their fp16 high and low parts (pairs, x in the low half)
+// x and y as their fp16 high and low parts (pairs, x in the low half); the low
+// part x - hi is exact in fp32 before its own rounding
 __device__ __forceinline__ void rt_split2(float x, float y, uint32_t& hi, uint32_t& lo)
 {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 hf = __half22float2(h);
-    const float2 r = fma2_rn(hf, make_float2(-1.0f, -1.0f), make_float2(x, y)); // exact
-    const __half2 l = __floats2half2_rn(r.x, r.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
+    float rx, ry;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+    asm("{\n\t.reg .b16 a, b, m;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 m, 0xBC00;\n\t" // m = -1
+        "fma.rn.f32.f16 %0, a, m, %3;\n\tfma.rn.f32.f16 %1, b, m, %4;\n\t}"
+        : "=f"(rx), "=f"(ry)
+        : "r"(hi), "f"(x), "f"(y));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
 }
 
-// max(m, |x|, |y|, |z|, |w|); a NaN stays
+// p[0..7] = v[0..7] * by, p 32-byte aligned
+__device__ __forceinline__ void rt_store8(float* p, const float* v, float by)
+{
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0] * by), "f"(v[1] * by),
+                 "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by), "f"(v[7] * by)
+                 : "memory");
+}
+
+// max(m, |x|, |y|); a NaN stays
+__device__ __forceinline__ float rt_max_abs(float m, float x, float y)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(x)), "f"(fabsf(y)));
+    return r;
+}
 __device__ __forceinline__ float rt_max_abs(float m, const float4& v)
 {
-    float a = m;
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.x)));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.y)));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.z)));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(v.w)));
-    return a;
+    return rt_max_abs(rt_max_abs(m, v.x, v.y), v.z, v.w);
 }
 
 // The power of two that puts a magnitude with these bits at 2^14..2^15, and
@@ -450,6 +437,27 @@ __device__ __forceinline__ void rt_regs_dec()
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
+// Waits for the phase with the given parity; false: another role gave up, or
+// 2^22 tries (of up to a microsecond each) ran out. No clock and no call, to
+// keep the many waits small.
+__device__ __forceinline__ bool rt_wait(uint32_t bar, uint32_t parity, const volatile uint32_t* abort)
+{
+    for (uint32_t n = 0; n < (1u << 22); ++n)
+    {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(bar), "r"(parity)
+                     : "memory");
+        if (ok)
+            return true;
+        if (*abort)
+            return false;
+    }
+    return false;
+}
+
 struct RtUnitInfo
 {
     float k_down, v_down;      // what undoes the unit's scaling of K and V
@@ -460,16 +468,42 @@ struct RtUnitInfo
 struct RtShared
 {
     uint64_t raw[8], conv[8], free_[8]; // per stage: copied, converted, read by the MMAs
-    uint64_t s_full[2], p_full[2], o_full, o_empty, q_full[2], q_empty[2], done;
+    uint64_t s_full[2], p_full[2], o_full, o_empty, q_raw[4], q_full[2], q_empty[2], done;
     uint32_t tmem, abort;
     RtStart start;
     int stage_valid[8];
-    uint32_t wmax[2][8];
+    alignas(16) uint32_t wmax[2][8];
     RtUnitInfo info[RT_INFO];
     float alpha[4][128];
     float q_down[4][128]; // what undoes an item's rows' scaling of Q
+    uint64_t seen[4][128]; // which of a unit's keys a row attends
     float2 stats[4][128]; // (sum, offset) of an item's rows
 };
+
+// i / G for i < 128 and G <= 64, by the reciprocal in 2^-16 (kernel-wide
+// constant; the product's excess is below 1 / G)
+__device__ __forceinline__ int rt_div(int i, int G)
+{
+    return (int)(((uint32_t)i * ((65535u + (uint32_t)G) / (uint32_t)G)) >> 16);
+}
+
+// Where row i of a tile is in q or out (floats from the base; ld floats a
+// packed row), or -1 for a row without a token.
+__device__ __forceinline__ long long rt_row_at(const RtSeq& q, int h, int t, int i, int G, int R, size_t ld, int hd)
+{
+    const int tok = rt_div(i, G), r = t * R + tok;
+    if (tok >= R || r >= q.n)
+        return -1;
+    return (long long)((size_t)(q.begin + r) * ld + (size_t)(h * G + i - tok * G) * hd);
+}
+
+// scores of keys that a row does not attend
+__device__ __forceinline__ void rt_mask16(float (&s)[16], uint32_t seen)
+{
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        s[j] = (seen >> j) & 1u ? s[j] : -INFINITY;
+}
 
 // Which of the 64 keys of a unit a row attends. limit: causal: the row's last
 // slot; tree: past. nodes: tree: the sequence's nodes (mask bits that count).
@@ -523,23 +557,9 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
         *abort = 1u;
         atomicExch(err, 1u);
     };
-    // bounded; gives up at once when another role gave up
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-        if (mbar_try_wait(bar, parity))
-            return true;
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(bar, parity))
-        {
-            if (*abort)
-                return false;
-            if (globaltimer_ns() - t0 > RT_WAIT_LIMIT_NS)
-            {
-                fail();
-                return false;
-            }
-        }
-        return true;
-    };
+    // false: the role ends (and says so in `failed`), and with it all others
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return rt_wait(bar, parity, abort); };
+    bool failed = false;
 
     if (warp == 0)
     {
@@ -567,8 +587,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 mbar_init(smem_addr(&sm.q_full[i]), 4);
                 mbar_init(smem_addr(&sm.q_empty[i]), 1);
             }
+            for (int i = 0; i < 4; ++i)
+                mbar_init(smem_addr(&sm.q_raw[i]), 1);
             mbar_init(smem_addr(&sm.o_full), 1);
-            mbar_init(smem_addr(&sm.o_empty), 4);
+            mbar_init(smem_addr(&sm.o_empty), 8);
             mbar_init(smem_addr(&sm.done), 1);
             mbar_init_fence();
             sm.abort = 0u;
@@ -651,7 +673,8 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             if (lane == 0)
             {
                 if (ok && due)
-                    emit(a.v, vpage, vh, vvalid);
+                    ok = emit(a.v, vpage, vh, vvalid);
+                failed = !ok;
                 // the copies it issued have landed before the CTA may exit
                 for (uint32_t p = pos > NS ? pos - NS : 0; p < pos; ++p)
                     mbar_wait_bounded(bar_raw(p), phase(p), RT_WAIT_LIMIT_NS);
@@ -673,7 +696,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 {
                     const uint32_t qb = item & 1u;
                     if ((u == c.u0 && !wait_all(smem_addr(&sm.q_full[qb]), (item >> 1) & 1u)) || !wait_all(bar_conv(pos), phase(pos)))
+                    {
+                        ok = false;
                         break;
+                    }
                     rt_fence_after();
                     const uint32_t k_hi = rt_desc_lo(stage_at(pos), 16u), d = RT_T_S + (g & 1u) * 64u;
                     const bool last = u + 1 == c.u1;
@@ -700,7 +726,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     const uint32_t j = g - 1u;
                     if (!wait_all(bar_conv(pos), phase(pos)) || !wait_all(smem_addr(&sm.p_full[j & 1u]), (j >> 1) & 1u) ||
                         (j >= 1u && !wait_all(smem_addr(&sm.o_empty), (j - 1u) & 1u)))
+                    {
+                        ok = false;
                         break;
+                    }
                     rt_fence_after();
                     const uint32_t v_hi = rt_desc_lo(stage_at(pos), 8192u), ph = RT_T_S + (j & 1u) * 64u;
                     if (rt_elect())
@@ -708,10 +737,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
 #pragma unroll 1
                         for (uint32_t p = 0; p < 3; ++p) // p_hi v_lo, p_lo v_hi, p_hi v_hi
                         {
-                            const uint32_t w = ph + (p == 1 ? 32u : 0u), v = v_hi + (p == 0 ? NB * 512u : 0u);
+                            const uint32_t w = ph + (p == 1 ? 8u : 0u), v = v_hi + (p == 0 ? NB * 512u : 0u);
 #pragma unroll
                             for (uint32_t n = 0; n < 4; ++n)
-                                rt_mma(RT_T_O, w + n * 8u, v + n * 128u, RT_DESC_HI, id_pv, p | n);
+                                rt_mma(RT_T_O, w + n * 16u, v + n * 128u, RT_DESC_HI, id_pv, p | n);
                         }
                         rt_commit(smem_addr(&sm.o_full));
                         rt_commit(bar_free(pos));
@@ -729,12 +758,13 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     ++item;
                 }
             }
+            failed = !ok;
             if (rt_elect())
                 rt_commit(smem_addr(&sm.done)); // every MMA issued, whatever happened
             __syncwarp();
         }
     }
-    else if (warp < 8)
+    else if (warp < RT_W_O)
     {
         // ---- softmax: thread = row
         rt_regs_inc<RT_REGS_SM>();
@@ -767,52 +797,58 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 const uint32_t ts = tmem + lanes + RT_T_S + b * 64u;
                 if (u == c.u0)
                     qf = qs * sm.q_down[item & 3u][i];
-                float s[64];
-                rt_ld<64>(ts, s);
                 const RtUnitInfo& in = sm.info[g % RT_INFO];
                 const float f = fmaxf(qf * in.k_down, 1.17549435e-38f);
                 const uint64_t seen = live ? rt_seen<TREE>(u, in.valid, limit, mask, a.mask_words) : 0ull;
+                sm.seen[g & 3u][i] = seen;
                 if ((in.kbad[0] | in.kbad[1]) != 0u &&
                     (seen & ((uint64_t)in.kbad[0] | (uint64_t)in.kbad[1] << 32)) != 0ull)
                     bad = true;
-                if (!__all_sync(0xffffffffu, seen == ~0ull))
+                const bool all = __all_sync(0xffffffffu, seen == ~0ull);
+                // 16 keys at a time, twice: the largest score, then the weights
+                // (P takes the place of S: 8 columns of high, 8 of low parts)
+                float s[16], m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll 1
+                for (uint32_t j0 = 0; j0 < 64; j0 += 16)
                 {
-                    const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
+                    rt_ld<16>(ts + j0, s);
+                    if (!all)
+                        rt_mask16(s, (uint32_t)(seen >> j0));
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
+                    for (int j = 0; j < 16; j += 4)
                     {
-                        s[j] = (s0 >> j) & 1u ? s[j] : -INFINITY;
-                        s[32 + j] = (s1 >> j) & 1u ? s[32 + j] : -INFINITY;
+                        m0 = fmaxf(m0, fmaxf(s[j], s[j + 1]));
+                        m1 = fmaxf(m1, fmaxf(s[j + 2], s[j + 3]));
                     }
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int j = 4; j < 64; ++j)
-                    mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const float noff = fminf(off, 14.0f - top * f);
+                const float noff = fminf(off, 14.0f - fmaxf(m0, m1) * f);
                 const float use = noff < INFINITY ? noff : 0.0f;
                 const float corr = rt_exp2(use - off); // 0 before the first key
                 off = noff;
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                float2 sum = make_float2(0.f, 0.f);
                 const float2 f2 = make_float2(f, f), use2 = make_float2(use, use);
-#pragma unroll
-                for (int j0 = 0; j0 < 4; ++j0)
+#pragma unroll 1
+                for (uint32_t j0 = 0; j0 < 64; j0 += 16)
                 {
+                    rt_ld<16>(ts + j0, s);
+                    if (!all)
+                        rt_mask16(s, (uint32_t)(seen >> j0));
                     uint32_t hi[8], lo[8];
+                    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                     {
-                        float2 x = fma2_rn(make_float2(s[j0 * 16 + 2 * j], s[j0 * 16 + 2 * j + 1]), f2, use2);
+                        float2 x = fma2_rn(make_float2(s[2 * j], s[2 * j + 1]), f2, use2);
                         x.x = rt_exp2(x.x);
                         x.y = rt_exp2(x.y);
-                        sum[j & 1] = rt_add2(sum[j & 1], x);
+                        part[j & 1] = rt_add2(part[j & 1], x);
                         rt_split2(x.x, x.y, hi[j], lo[j]);
                     }
-                    rt_st8(ts + j0 * 8, hi);
-                    rt_st8(ts + 32 + j0 * 8, lo);
+                    sum = rt_add2(sum, rt_add2(part[0], part[1]));
+                    rt_st8(ts + j0, hi);
+                    rt_st8(ts + j0 + 8, lo);
                 }
-                l = fmaf(l, corr, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                l = fmaf(l, corr, sum.x + sum.y);
                 sm.alpha[g & 3u][i] = corr;
                 if (u + 1 == c.u1)
                     sm.stats[item & 3u][i] = make_float2(bad ? __uint_as_float(0x7FC00000u) : l, off);
@@ -823,25 +859,26 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     mbar_arrive(smem_addr(&sm.p_full[b]));
             }
         }
+        failed = !ok;
     }
-    else if (warp < 12)
+    else if (warp < RT_W_CV)
     {
-        // ---- output sums: thread = row
+        // ---- output sums: thread = row, a warpgroup for each half of the dims
         rt_regs_inc<RT_REGS_O>();
-        const int i = (warp & 3) * 32 + lane, ti = i / G, gi = i - ti * G;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        constexpr int W = HDP / 2;
+        const int i = (warp & 3) * 32 + lane, d_first = warp < RT_W_O + 4 ? 0 : W;
+        const uint32_t t_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + RT_T_O + d_first;
         uint32_t g = 0, item = 0;
         bool ok = true;
         RtCursor<TREE> c;
         for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
         {
-            const int r = c.t * R + ti;
-            const bool live = ti < R && r < c.q.n;
-            float acc[HDP];
+            float acc[W]; // in units of `unit`, the largest scale of V so far
 #pragma unroll
-            for (int d = 0; d < HDP; ++d)
+            for (int d = 0; d < W; ++d)
                 acc[d] = 0.0f;
             float2 stat = make_float2(0.0f, INFINITY);
+            float unit = 0.0f;
             bool bad = false;
             for (int u = c.u0; u < c.u1; ++u, ++g)
             {
@@ -851,29 +888,33 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     break;
                 }
                 rt_fence_after();
-                const float corr = sm.alpha[g & 3u][i];
+                float corr = sm.alpha[g & 3u][i];
                 const RtUnitInfo& in = sm.info[g % RT_INFO];
-                const float f = in.v_down;
-                if ((in.vbad[0] | in.vbad[1]) != 0u && live)
-                {
-                    const uint64_t seen = rt_seen<TREE>(
-                        u, in.valid, TREE ? c.q.past : min(c.q.past, INT_MAX - c.q.n) + r,
-                        TREE ? a.mask + (size_t)(c.q.begin + r) * a.mask_words : nullptr, a.mask_words);
-                    bad |= (seen & ((uint64_t)in.vbad[0] | (uint64_t)in.vbad[1] << 32)) != 0ull;
-                }
+                if ((in.vbad[0] | in.vbad[1]) != 0u)
+                    bad |= (sm.seen[g & 3u][i] & ((uint64_t)in.vbad[0] | (uint64_t)in.vbad[1] << 32)) != 0ull;
                 if (u + 1 == c.u1)
                     stat = sm.stats[item & 3u][i];
-                const float2 c2 = make_float2(corr, corr), f2 = make_float2(f, f);
+                const float f = in.v_down; // a power of two, the same for all rows
+                if (f > unit)
+                {
+                    corr *= unit / f; // exact, or an underflow of sums that no longer count
+                    unit = f;
+                }
+                const float2 c2 = make_float2(corr, corr);
+                const float down = f / unit;
 #pragma unroll
-                for (int d0 = 0; d0 < HDP; d0 += 16)
+                for (int d0 = 0; d0 < W; d0 += 16)
                 {
                     float t[16];
-                    rt_ld<16>(tmem + lanes + RT_T_O + d0, t);
+                    rt_ld<16>(t_o + d0, t);
+                    if (down != 1.0f)
+#pragma unroll
+                        for (int d = 0; d < 16; ++d)
+                            t[d] *= down;
 #pragma unroll
                     for (int d = 0; d < 16; d += 2)
                     {
-                        const float2 x = mul2_rn(make_float2(t[d], t[d + 1]), f2);
-                        const float2 y = fma2_rn(make_float2(acc[d0 + d], acc[d0 + d + 1]), c2, x);
+                        const float2 y = fma2_rn(make_float2(acc[d0 + d], acc[d0 + d + 1]), c2, make_float2(t[d], t[d + 1]));
                         acc[d0 + d] = y.x;
                         acc[d0 + d + 1] = y.y;
                     }
@@ -886,55 +927,91 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             if (!ok)
                 break;
             const float l = bad ? __uint_as_float(0x7FC00000u) : stat.x;
+            float* to;
+            float by = unit;
+            int n = W; // dims to store
             if (c.whole)
             {
-                if (live)
-                {
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    float4* o = reinterpret_cast<float4*>(a.out + (size_t)(c.q.begin + r) * a.ldo + (size_t)(c.h * G + gi) * hd);
-#pragma unroll
-                    for (int d = 0; d < HDP; d += 4)
-                        if (d < hd)
-                            o[d / 4] = make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
-                }
+                const long long at = rt_row_at(c.q, c.h, c.t, i, G, R, a.ldo, hd);
+                to = a.out + at + d_first;
+                by = l == 0.0f ? 0.0f : unit / l;
+                n = at < 0 ? 0 : hd - d_first;
             }
             else
             {
                 float* slot = rt_slot<HDP>(a, blockIdx.x, item == 0 ? 0 : 1);
-                float4* o = reinterpret_cast<float4*>(slot + (size_t)i * HDP);
+                to = slot + (size_t)i * HDP + d_first;
+                if (d_first == 0)
+                    reinterpret_cast<float2*>(slot + 128 * HDP)[i] = make_float2(l, stat.y);
+            }
+            // a row a thread: whole 32-byte sectors where the addresses allow it
+            if (((uint32_t)reinterpret_cast<uintptr_t>(to) & 31u) == 0u && (n & 7) == 0)
+            {
 #pragma unroll
-                for (int d = 0; d < HDP; d += 4)
-                    o[d / 4] = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-                reinterpret_cast<float2*>(slot + 128 * HDP)[i] = make_float2(l, stat.y);
+                for (int d = 0; d < W; d += 8)
+                    if (d < n)
+                        rt_store8(to + d, acc + d, by);
+            }
+            else
+            {
+#pragma unroll
+                for (int d = 0; d < W; d += 4)
+                    if (d < n)
+                        *reinterpret_cast<float4*>(to + d) =
+                            make_float4(acc[d] * by, acc[d + 1] * by, acc[d + 2] * by, acc[d + 3] * by);
             }
         }
+        failed = !ok;
     }
-    else if (warp < 20)
+    else if (warp < RT_W_Q)
     {
         // ---- a stage from fp32 to its fp16 parts, in place
         rt_regs_dec<RT_REGS_CV>();
-        const int ct = tid - 12 * 32, cw = ct >> 5;
+        const int ct = tid - RT_W_CV * 32, cw = ct >> 5;
         constexpr int NCH = 64 * HDP / 4 / RT_CONV_THREADS; // 16-byte pieces a thread
-        uint32_t pos = 0;
+        constexpr int PR = HDP / 4, RS = RT_CONV_THREADS / PR; // pieces a row, rows from one piece of a thread to its next
+        const int row0 = ct / PR, col = ct % PR;
+        const bool in_row = col * 4 < hd;
+        const uint32_t in_off = (uint32_t)(row0 * hd + col * 4) * 4u, in_step = (uint32_t)(RS * hd) * 4u;
+        // its place in the swizzled rows (RS is a multiple of 8: the same swizzle for every piece)
+        const int e = (col & 15) * 4; // element of the 64-dim block
+        const uint32_t out_off = (uint32_t)(col >> 4) * 8192u + (uint32_t)row0 * 128u +
+                                 (uint32_t)(((e >> 3) ^ (row0 & 7)) * 16 + (e & 7) * 2);
+        uint32_t slot = 0, ph = 0, par = 0;
         auto convert = [&](uint32_t unit, bool is_k) -> bool {
-            const bool got = wait(bar_raw(pos), phase(pos));
-            const uint32_t stage = stage_at(pos), par = pos & 1u;
+            const bool got = wait(smem_addr(&sm.raw[slot]), ph);
+            const uint32_t stage = ring + slot * Cfg::STAGE;
             RtUnitInfo& in = sm.info[unit % RT_INFO];
-            const int valid = got ? sm.stage_valid[pos % NS] : 0;
+            const int valid = got ? sm.stage_valid[slot] : 0;
             float4 x[NCH];
-            float mx = 0.0f; // NaN is kept
+            float mx = 0.0f, my = 0.0f; // NaN is kept
+            if (valid == 64 && hd == HDP)
+            {
+#pragma unroll
+                for (int n = 0; n < NCH; ++n)
+                {
+                    const uint4 w = lds128(stage + in_off + n * in_step);
+                    x[n] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int n = 0; n < NCH; ++n)
+                {
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u); // behind the last key, behind head_dim
+                    if (in_row && row0 + n * RS < valid)
+                        w = lds128(stage + in_off + n * in_step);
+                    x[n] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NCH; ++n)
             {
-                const int f = n * RT_CONV_THREADS + ct, row = f / (HDP / 4), c = f % (HDP / 4);
-                x[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (row < valid && c * 4 < hd)
-                {
-                    const uint4 w = lds128(stage + (uint32_t)(row * hd + c * 4) * 4u);
-                    x[n] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
-                }
-                mx = rt_max_abs(mx, x[n]);
+                mx = rt_max_abs(mx, x[n].x, x[n].y);
+                my = rt_max_abs(my, x[n].z, x[n].w);
             }
+            mx = rt_max_abs(mx, my, 0.0f);
             if (!(mx < INFINITY))
             {
                 // NaN or infinity: the key is noted and its values are zeros
@@ -944,24 +1021,23 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 {
                     if (!(rt_max_abs(0.0f, x[n]) < INFINITY))
                     {
-                        const int row = (n * RT_CONV_THREADS + ct) / (HDP / 4);
+                        const int row = row0 + n * RS;
                         atomicOr(is_k ? &in.kbad[row >> 5] : &in.vbad[row >> 5], 1u << (row & 31));
                         x[n] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
                     mx = rt_max_abs(mx, x[n]);
                 }
             }
-            uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)); // not negative: ordered as integers
+            const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)); // not negative: ordered as integers
             if (lane == 0)
-                sm.wmax[par][cw] = mb;
+                sm.wmax[par][cw] = wm;
             // every read of the stage is done; a failed wait ends all eight warps together
             if (named_bar_or(1, RT_CONV_THREADS, !got))
                 return false;
-#pragma unroll
-            for (int w = 0; w < RT_CONV_THREADS / 32; ++w)
-                mb = max(mb, sm.wmax[par][w]);
+            const uint4 m0 = *reinterpret_cast<const uint4*>(&sm.wmax[par][0]);
+            const uint4 m1 = *reinterpret_cast<const uint4*>(&sm.wmax[par][4]);
             float up, down;
-            rt_scale_of(mb, up, down);
+            rt_scale_of(max(max(max(m0.x, m0.y), max(m0.z, m0.w)), max(max(m1.x, m1.y), max(m1.z, m1.w))), up, down);
             if (ct == 0)
             {
                 if (is_k)
@@ -975,24 +1051,28 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 else
                     in.v_down = down;
             }
+            const float2 up2 = make_float2(up, up);
 #pragma unroll
             for (int n = 0; n < NCH; ++n)
             {
-                const int f = n * RT_CONV_THREADS + ct, row = f / (HDP / 4), c = f % (HDP / 4);
                 uint32_t h0, l0, h1, l1;
-                rt_split2(x[n].x * up, x[n].y * up, h0, l0);
-                rt_split2(x[n].z * up, x[n].w * up, h1, l1);
-                const int e = (c & 15) * 4; // element of the 64-dim block
-                const uint32_t at = stage + (uint32_t)(c >> 4) * 8192u + (uint32_t)row * 128u +
-                                    (uint32_t)(((e >> 3) ^ (row & 7)) * 16 + (e & 7) * 2);
+                const float2 a2 = mul2_rn(make_float2(x[n].x, x[n].y), up2), b2 = mul2_rn(make_float2(x[n].z, x[n].w), up2);
+                rt_split2(a2.x, a2.y, h0, l0);
+                rt_split2(b2.x, b2.y, h1, l1);
+                const uint32_t at = stage + out_off + n * (RS * 128u);
                 asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(h0), "r"(h1) : "memory");
                 asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + NB * 8192u), "r"(l0), "r"(l1) : "memory");
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the MMA reads through the async proxy
             __syncwarp();
             if (lane == 0)
-                mbar_arrive(bar_conv(pos));
-            ++pos;
+                mbar_arrive(smem_addr(&sm.conv[slot]));
+            par ^= 1u;
+            if (++slot == NS)
+            {
+                slot = 0;
+                ph ^= 1u;
+            }
             return true;
         };
         // K of every unit, each followed by V of the unit before; the last V
@@ -1004,60 +1084,85 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             const bool is_k = e == 1u || (!(e & 1u) && e < 2u * left);
             ok = convert(is_k ? e >> 1 : (e == 2u * left ? left - 1u : (e - 3u) >> 1), is_k);
         }
+        failed = !ok;
     }
     else
     {
-        // ---- the next tile's queries into tensor memory: thread = row
+        // ---- queries: bulk copies bring the next tile's rows to shared memory
+        // while this one's go to tensor memory; thread = row
         rt_regs_dec<RT_REGS_Q>();
-        const int i = (warp & 3) * 32 + lane, ti = i / G, gi = i - ti * G;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int w = warp & 3, i = w * 32 + lane;
+        const uint32_t lanes = (uint32_t)(w * 32) << 16;
+        const uint32_t row = ring + NS * Cfg::STAGE + (uint32_t)i * Cfg::Q_ROW, raw = smem_addr(&sm.q_raw[w]);
         const float sign = a.scale < 0.0f ? -1.0f : 1.0f; // the softmax takes |scale|
         uint32_t item = 0;
         bool ok = true;
         RtCursor<TREE> c;
-        for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
+        auto copy = [&]() -> bool { // true: the row has a token
+            const long long at = rt_row_at(c.q, c.h, c.t, i, G, R, a.ldq, hd);
+            const uint32_t n = __popc(__ballot_sync(0xffffffffu, at >= 0));
+            if (lane == 0)
+                mbar_arrive_expect_tx(raw, n * (uint32_t)hd * 4u);
+            __syncwarp();
+            if (at >= 0)
+                bulk_g2s(row, a.q + at, (uint32_t)hd * 4u, raw);
+            return at >= 0;
+        };
+        bool more = c.start(a, st0, share, R), live = more && copy();
+        for (; more; ++item)
         {
             const uint32_t qb = item & 1u;
-            const int r = c.t * R + ti;
-            const bool live = ti < R && r < c.q.n;
-            const float4* qr = reinterpret_cast<const float4*>(a.q + (size_t)(c.q.begin + (live ? r : 0)) * a.ldq +
-                                                               (size_t)(c.h * G + gi) * hd);
-            float mx = 0.0f; // NaN is kept
-            if (live)
-#pragma unroll 4
-                for (int d = 0; d < hd / 4; ++d)
-                    mx = rt_max_abs(mx, qr[d]);
-            float q_up, q_down;
-            rt_scale_of(__float_as_uint(mx) & 0x7FFFFFFFu, q_up, q_down);
-            q_up *= sign;
-            if (item >= 2 && !wait_all(smem_addr(&sm.q_empty[qb]), ((item >> 1) & 1u) ^ 1u))
+            if (!wait_all(raw, item & 1u) ||
+                (item >= 2 && !wait_all(smem_addr(&sm.q_empty[qb]), ((item >> 1) & 1u) ^ 1u)))
             {
                 ok = false;
                 break;
             }
             rt_fence_after();
+            float mx = 0.0f; // NaN is kept
+            if (live)
+#pragma unroll 4
+                for (int d = 0; d < hd; d += 4)
+                {
+                    const uint4 x = lds128(row + (uint32_t)d * 4u);
+                    mx = rt_max_abs(mx, make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z),
+                                                    __uint_as_float(x.w)));
+                }
+            float q_up, q_down;
+            rt_scale_of(__float_as_uint(mx) & 0x7FFFFFFFu, q_up, q_down);
+            q_up *= sign;
             sm.q_down[item & 3u][i] = q_down;
 #pragma unroll 1
-            for (int d0 = 0; d0 < HDP / 16; ++d0)
+            for (int d0 = 0; d0 < HDP; d0 += 16)
             {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
                 {
-                    const float4 x = live && (d0 * 4 + d) * 4 < hd ? qr[d0 * 4 + d] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    rt_split2(x.x * q_up, x.y * q_up, hi[2 * d], lo[2 * d]);
-                    rt_split2(x.z * q_up, x.w * q_up, hi[2 * d + 1], lo[2 * d + 1]);
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (live && d0 + d * 4 < hd)
+                        x = lds128(row + (uint32_t)(d0 + d * 4) * 4u);
+                    rt_split2(__uint_as_float(x.x) * q_up, __uint_as_float(x.y) * q_up, hi[2 * d], lo[2 * d]);
+                    rt_split2(__uint_as_float(x.z) * q_up, __uint_as_float(x.w) * q_up, hi[2 * d + 1], lo[2 * d + 1]);
                 }
-                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + d0 * 8, hi);
-                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + (HDP == 128 ? RT_T_QLO : 32u) + d0 * 8, lo);
+                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + d0 / 2, hi);
+                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + (HDP == 128 ? RT_T_QLO : 32u) + d0 / 2, lo);
             }
             rt_wait_st();
             rt_fence_before();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the next copy overwrites what was read
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(smem_addr(&sm.q_full[qb]));
+            more = c.next(a, R);
+            live = more && copy();
         }
+        if (!ok) // a copy may be in flight: it has landed before the CTA exits
+            mbar_wait_bounded(raw, item & 1u, RT_WAIT_LIMIT_NS);
+        failed = !ok;
     }
+    if (failed && lane == 0)
+        fail();
     rt_fence_before();
     __syncthreads();
     if (warp == 1)
