@@ -7,6 +7,7 @@
 #include "common.cuh"
 
 #include "attn_rows.h"
+#include "gemm_tc.h" // tc_encode_fn
 #include "device_check.hpp"
 
 namespace aaedn_dev
@@ -50,6 +51,7 @@ __device__ __forceinline__ const int* rows_page_table(const AttnRowsArgs& a, int
 
 } // namespace aaedn_dev
 
+#include "attn_rows_pair.cuh"
 #include "attn_rows_tc.cuh"
 
 namespace aaedn_dev
@@ -153,15 +155,14 @@ __global__ void __launch_bounds__(RW_WARPS * 32) attn_rows_warp_kernel(const Att
             o[lane + 32 * i] = acc[i] * inv;
 }
 
-template <int HDP, bool TREE>
-static int rows_tc_attrs()
+template <typename Kern>
+static int rows_tc_attrs(Kern kern, size_t smem)
 {
-    auto kern = attn_rows_tc_kernel<HDP, TREE>;
-    AAEDN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RtCfg<HDP>::SMEM));
+    AAEDN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaFuncAttributes at;
     AAEDN_CUDA_TRY(cudaFuncGetAttributes(&at, kern));
     if (at.numRegs != RT_REGS) // the roles' register shares are drawn from the launch's
-        return set_error(AAEDN_EUNSUPPORTED, "attn_rows_tc_kernel built with %d registers, not %d", at.numRegs, RT_REGS);
+        return set_error(AAEDN_EUNSUPPORTED, "an attn_rows kernel was built with %d registers, not %d", at.numRegs, RT_REGS);
     return AAEDN_OK;
 }
 
@@ -170,33 +171,103 @@ int attn_rows_init()
     static PerDeviceOnce once;
     return once.run([]() -> int {
         int rc;
-        if ((rc = rows_tc_attrs<64, false>()) || (rc = rows_tc_attrs<64, true>()) || (rc = rows_tc_attrs<128, false>()))
+        if ((rc = rows_tc_attrs(attn_rows_tc_kernel<64, false>, RtCfg<64>::SMEM)) ||
+            (rc = rows_tc_attrs(attn_rows_tc_kernel<64, true>, RtCfg<64>::SMEM)) ||
+            (rc = rows_tc_attrs(attn_rows_pair_kernel<false>, RP_SMEM)))
             return rc;
-        return rows_tc_attrs<128, true>();
+        return rows_tc_attrs(attn_rows_pair_kernel<true>, RP_SMEM);
     });
+}
+
+// the word that a bounded wait's failure sets
+static int rows_err_word(const AttnRowsArgs& a, unsigned** err)
+{
+    *err = a.err;
+    if (!a.err)
+    {
+        void* p = nullptr;
+        AAEDN_CUDA_TRY(cudaGetSymbolAddress(&p, g_attn_rows_err));
+        *err = static_cast<unsigned*>(p);
+    }
+    return AAEDN_OK;
+}
+
+// CTAs of a launch: one an SM, as far as the workspace's partial sums go
+template <int HDP>
+static int rows_grid()
+{
+    return std::min<int>(sm_count(), (int)((AAEDN_ATTN_ROWS_WORKSPACE_BYTES - RT_HEADER_BYTES) / (2 * rt_slot_bytes<HDP>())));
+}
+
+// The tensor map of a page pool as rows of head_dim floats, `dims` x `keys` a copy.
+static int rows_map(CUtensorMap& map, const AttnRowsArgs& a, const float* pool, int dims, int keys)
+{
+    const PFN_cuTensorMapEncodeTiled_v12000 enc = tc_encode_fn();
+    if (!enc)
+        return set_error(AAEDN_ECUDA, "packed attention: cuTensorMapEncodeTiled is not available");
+    const cuuint64_t size[2] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.n_pages * (cuuint64_t)a.n_kv * ROWS_PAGE};
+    const cuuint64_t stride[1] = {(cuuint64_t)a.head_dim * 4};
+    const cuuint32_t box[2] = {(cuuint32_t)dims, (cuuint32_t)keys};
+    const cuuint32_t one[2] = {1, 1};
+    const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(pool), size, stride, box, one,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(AAEDN_ECUDA, "packed attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return AAEDN_OK;
+}
+
+template <int HDP, bool TREE, int NC>
+static int rows_join(const AttnRowsArgs& a, int shares, cudaStream_t st)
+{
+    if (shares < 2)
+        return AAEDN_OK;
+    const cudaError_t e = launch_kernel(attn_rows_join_kernel<HDP, TREE, NC>, dim3((unsigned)shares - 1, NC * 128 / RJ_WARPS),
+                                        dim3(RJ_WARPS * 32), 0, st, true, a, shares);
+    if (e != cudaSuccess)
+        return set_error(AAEDN_ECUDA, "launch of attn_rows_join_kernel failed: %s", cudaGetErrorString(e));
+    count_launch();
+    return AAEDN_OK;
+}
+
+template <bool TREE>
+static int rows_pair_launch(const AttnRowsArgs& a, cudaStream_t st)
+{
+    unsigned* err;
+    CUtensorMap kmap, vmap;
+    int rc;
+    if ((rc = rows_err_word(a, &err)) || (rc = rows_map(kmap, a, a.k, 128, 32)) || (rc = rows_map(vmap, a, a.v, 64, 64)))
+        return rc;
+    const int pairs = rows_grid<RP_HDP>() / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)pairs);
+    cfg.blockDim = dim3(RT_THREADS);
+    cfg.dynamicSmemBytes = RP_SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_rows_pair_kernel<TREE>, a, err, kmap, vmap);
+    if (e != cudaSuccess)
+        return set_error(AAEDN_ECUDA, "launch of attn_rows_pair_kernel failed: %s", cudaGetErrorString(e));
+    count_launch();
+    return rows_join<RP_HDP, TREE, 2>(a, pairs, st);
 }
 
 template <int HDP, bool TREE>
 static int rows_tc_launch(const AttnRowsArgs& a, cudaStream_t st)
 {
-    unsigned* err = a.err;
-    if (!err)
-    {
-        void* p = nullptr;
-        AAEDN_CUDA_TRY(cudaGetSymbolAddress(&p, g_attn_rows_err));
-        err = static_cast<unsigned*>(p);
-    }
-    // one CTA an SM, as far as the workspace's partial sums go
-    const int grid = std::min<int>(sm_count(), (int)((AAEDN_ATTN_ROWS_WORKSPACE_BYTES - RT_HEADER_BYTES) /
-                                                     (2 * rt_slot_bytes<HDP>())));
+    unsigned* err;
+    if (int rc = rows_err_word(a, &err))
+        return rc;
+    const int grid = rows_grid<HDP>();
     attn_rows_tc_kernel<HDP, TREE><<<grid, RT_THREADS, RtCfg<HDP>::SMEM, st>>>(a, err);
     AAEDN_LAUNCH_CHECK("attn_rows_tc_kernel");
-    const cudaError_t e = launch_kernel(attn_rows_join_kernel<HDP, TREE>, dim3((unsigned)grid - 1, 128 / RJ_WARPS),
-                                        dim3(RJ_WARPS * 32), 0, st, true, a, grid);
-    if (e != cudaSuccess)
-        return set_error(AAEDN_ECUDA, "launch of attn_rows_join_kernel failed: %s", cudaGetErrorString(e));
-    count_launch();
-    return AAEDN_OK;
+    return rows_join<HDP, TREE, 1>(a, grid, st);
 }
 
 int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
@@ -207,7 +278,7 @@ int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
             return rc;
         if (a.head_dim <= 64)
             return a.mask ? rows_tc_launch<64, true>(a, st) : rows_tc_launch<64, false>(a, st);
-        return a.mask ? rows_tc_launch<128, true>(a, st) : rows_tc_launch<128, false>(a, st);
+        return a.mask ? rows_pair_launch<true>(a, st) : rows_pair_launch<false>(a, st);
     }
     const dim3 grid((unsigned)((a.rows + RW_WARPS - 1) / RW_WARPS), (unsigned)a.n_heads);
     if (a.mask)

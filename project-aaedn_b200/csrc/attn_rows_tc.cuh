@@ -1182,7 +1182,8 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
 // ---------------------------------------------------------------------------
 constexpr int RJ_WARPS = 8;
 
-template <int HDP, bool TREE>
+// NC CTAs work on a share together (128 rows each).
+template <int HDP, bool TREE, int NC>
 __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const AttnRowsArgs a, int grid)
 {
     pdl_wait();
@@ -1195,12 +1196,13 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
     const unsigned long long t0 = st.begin - (unsigned)st.u;
     if (rt_share(st.total, c0 - 1, grid) > t0)
         return;
-    const int G = a.n_heads / a.n_kv, R = 128 / G, i = blockIdx.y * RJ_WARPS + (threadIdx.x >> 5), ti = i / G;
-    const RtSeq q = rt_seq(a, st.s, R);
-    const int r = st.t * R + ti;
+    const int G = a.n_heads / a.n_kv, R = 128 / G, i2 = blockIdx.y * RJ_WARPS + (threadIdx.x >> 5);
+    const int part = i2 >> 7, i = i2 & 127, ti = i / G; // CTA of the share, row of the CTA
+    const RtSeq q = rt_seq(a, st.s, NC * R);
+    const int r = (st.t * NC + part) * R + ti;
     if (ti >= R || r >= q.n)
         return;
-    const unsigned long long t1 = t0 + (unsigned)((rt_keys(q, TREE, R, st.t) + 63) / 64);
+    const unsigned long long t1 = t0 + (unsigned)((rt_keys(q, TREE, NC * R, st.t) + 63) / 64);
     // the first share with a unit of the tile: the last one that starts at or before it and is not empty
     int first = c0 - 1;
     while (first > 0 && rt_share(st.total, first, grid) > t0)
@@ -1215,7 +1217,7 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         const unsigned long long b = rt_share(st.total, c, grid);
         if (b >= t1 || rt_share(st.total, c + 1, grid) == b)
             return none;
-        return __ldcg(reinterpret_cast<const float2*>(rt_slot<HDP>(a, c, b >= t0 ? 0 : 1) + 128 * HDP) + i);
+        return __ldcg(reinterpret_cast<const float2*>(rt_slot<HDP>(a, c * NC + part, b >= t0 ? 0 : 1) + 128 * HDP) + i);
     };
     int last = first; // the last share with a unit of the tile
     {
@@ -1247,7 +1249,7 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         {
             const float wj = __shfl_sync(0xffffffffu, w, j);
             // an empty share (weight 0) has no sums: its slot is not read
-            const float* slot = rt_slot<HDP>(a, c + j, j > 0 || c > first || rt_share(st.total, first, grid) >= t0 ? 0 : 1);
+            const float* slot = rt_slot<HDP>(a, (c + j) * NC + part, j > 0 || c > first || rt_share(st.total, first, grid) >= t0 ? 0 : 1);
             const bool some = __shfl_sync(0xffffffffu, s.y, j) < INFINITY;
 #pragma unroll
             for (int d = 0; d < HDP / 32; ++d)

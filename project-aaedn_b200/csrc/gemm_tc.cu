@@ -12,10 +12,7 @@
 namespace aaedn_dev
 {
 
-namespace
-{
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
+PFN_cuTensorMapEncodeTiled_v12000 tc_encode_fn()
 {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -28,6 +25,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
     });
     return fn;
 }
+
+namespace
+{
 
 struct TcShape
 {
@@ -125,7 +125,7 @@ int tc_gemm(const TcGemmArgs& a, cudaStream_t st)
     if (!a.workspace || a.workspace_bytes < tc_gemm_workspace_bytes(a.M, a.N, a.K))
         return set_error(AAEDN_EINVAL, "tensor-core GEMM: workspace of %zu bytes, need %zu", a.workspace_bytes,
                          tc_gemm_workspace_bytes(a.M, a.N, a.K));
-    auto encode = encode_fn();
+    auto encode = tc_encode_fn();
     if (!encode)
         return set_error(AAEDN_ECUDA, "tensor-core GEMM: cuTensorMapEncodeTiled is not available");
     const TcShape sh = tc_shape(a.M);

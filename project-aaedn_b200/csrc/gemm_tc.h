@@ -3,6 +3,7 @@
 // scale(n, k / 32) for M activation rows, fp32 in and out, fp32-accurate.
 #pragma once
 
+#include <cudaTypedefs.h> // PFN_cuTensorMapEncodeTiled
 #include <cuda_runtime.h>
 
 #include <cstddef>
@@ -10,6 +11,9 @@
 
 namespace aaedn_dev
 {
+
+// cuTensorMapEncodeTiled of the driver, or null.
+PFN_cuTensorMapEncodeTiled_v12000 tc_encode_fn();
 
 // Order of the K elements inside every group of 8 in the GEMM's operands
 // (and so in the activation parts written for it): k = 4 h + j sits at
