@@ -238,9 +238,8 @@ static int rows_pair_launch(const AttnRowsArgs& a, cudaStream_t st)
     int rc;
     if ((rc = rows_err_word(a, &err)) || (rc = rows_map(kmap, a, a.k, 128, 32)) || (rc = rows_map(vmap, a, a.v, 64, 64)))
         return rc;
-    const int pairs = rows_grid<RP_HDP>() / 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)pairs);
+    cfg.gridDim = dim3(2 * (unsigned)(rows_grid<RP_HDP>() / 2));
     cfg.blockDim = dim3(RT_THREADS);
     cfg.dynamicSmemBytes = RP_SMEM;
     cfg.stream = st;
@@ -251,6 +250,21 @@ static int rows_pair_launch(const AttnRowsArgs& a, cudaStream_t st)
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    // as many pairs as run at once: the shares are equal, so one pair that
+    // waits for another's SMs would double the time (a GPU whose SMs do not
+    // all pair up inside their cluster groups holds fewer than SMs / 2)
+    static std::atomic<int> fit[64];
+    int dev = 0;
+    AAEDN_CUDA_TRY(cudaGetDevice(&dev));
+    std::atomic<int>& slot = fit[dev & 63];
+    int pairs = slot.load(std::memory_order_relaxed);
+    if (pairs <= 0)
+    {
+        AAEDN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&pairs, attn_rows_pair_kernel<TREE>, &cfg));
+        pairs = std::max(1, std::min(pairs, rows_grid<RP_HDP>() / 2));
+        slot.store(pairs, std::memory_order_relaxed);
+    }
+    cfg.gridDim = dim3(2 * (unsigned)pairs);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_rows_pair_kernel<TREE>, a, err, kmap, vmap);
     if (e != cudaSuccess)
         return set_error(AAEDN_ECUDA, "launch of attn_rows_pair_kernel failed: %s", cudaGetErrorString(e));

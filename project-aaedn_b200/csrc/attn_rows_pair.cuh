@@ -49,7 +49,7 @@ struct RpShared
     uint64_t raw[2][RP_NS], conv[2][RP_NS], free_[2][RP_NS]; // K, V stages: copied, converted, read by the MMAs
     uint64_t s_full[2], p_full[2], o_full, o_empty, q_raw[4], q_full[2], q_empty[2], done;
     uint32_t tmem, abort;
-    RtStart start;
+    RtStart start, end;
     int stage_valid[2][RP_NS];
     alignas(16) uint32_t wmax[2][2][4];
     uint32_t bad[2][2][2];
@@ -160,6 +160,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                 reinterpret_cast<RtStart*>(a.workspace)[pair] = st;
         }
     }
+    else if (warp == 3)
+    {
+        const RtStart en = rt_locate<TREE>(a, R2, pair + 1, pairs);
+        if (lane == 0)
+        {
+            sm.end = en;
+            if (rank == 0 && pair + 1 == pairs)
+                reinterpret_cast<RtStart*>(a.workspace)[pairs] = en;
+        }
+    }
     else if (warp == 1)
     {
         if (lane == 0)
@@ -205,7 +215,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
     rt_fence_after();
     constexpr uint32_t tmem = 0u; // all columns are the CTA's
     const RtStart st0 = sm.start;
-    unsigned long long share = rt_share(st0.total, pair + 1, pairs) - st0.begin;
+    unsigned long long share = sm.end.begin - st0.begin;
     if (sm.tmem != tmem) // cannot be: nothing runs on other columns
     {
         share = 0;
@@ -408,8 +418,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                 if ((in.y | in.w) != 0u && (seen & ((uint64_t)in.y | (uint64_t)in.w << 32)) != 0ull)
                     bad = true;
                 const bool all = __all_sync(0xffffffffu, seen == ~0ull);
-                // 16 keys at a time, twice: the largest score, then the weights
-                // (P takes the place of S: 8 columns of high, 8 of low parts)
+                // 16 keys at a time, twice: the largest score, then the weights (P takes
+                // the place of S). Rolled loops over tensor memory: with all 64
+                // scores in registers a unit alone is faster, the kernel 13 % slower
+                // (its roles' code no longer fits the instruction caches).
                 float s[16], top = -INFINITY;
 #pragma unroll 1
                 for (uint32_t j0 = 0; j0 < 64; j0 += 16)
@@ -417,43 +429,20 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                     rt_ld<16>(ts + j0, s);
                     if (!all)
                         rt_mask16(s, (uint32_t)(seen >> j0));
-                    float m0 = s[0], m1 = s[1];
-#pragma unroll
-                    for (int j = 2; j < 16; j += 2)
-                    {
-                        m0 = fmaxf(m0, s[j]);
-                        m1 = fmaxf(m1, s[j + 1]);
-                    }
-                    top = fmaxf(top, fmaxf(m0, m1) * (j0 < 32 ? fa : fb));
+                    top = fmaxf(top, rt_max16(s) * (j0 < 32 ? fa : fb));
                 }
                 const float noff = fminf(off, 14.0f - top);
                 const float use = noff < INFINITY ? noff : 0.0f;
                 const float corr = rt_exp2(use - off); // 0 before the first key
                 off = noff;
                 float2 sum = make_float2(0.f, 0.f);
-                const float2 use2 = make_float2(use, use);
 #pragma unroll 1
                 for (uint32_t j0 = 0; j0 < 64; j0 += 16)
                 {
                     rt_ld<16>(ts + j0, s);
                     if (!all)
                         rt_mask16(s, (uint32_t)(seen >> j0));
-                    const float f = j0 < 32 ? fa : fb;
-                    const float2 f2 = make_float2(f, f);
-                    uint32_t hi[8], lo[8];
-                    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                    {
-                        float2 x = fma2_rn(make_float2(s[2 * j], s[2 * j + 1]), f2, use2);
-                        x.x = rt_exp2(x.x);
-                        x.y = rt_exp2(x.y);
-                        part[j & 1] = rt_add2(part[j & 1], x);
-                        rt_split2(x.x, x.y, hi[j], lo[j]);
-                    }
-                    sum = rt_add2(sum, rt_add2(part[0], part[1]));
-                    rt_st8(ts + j0, hi);
-                    rt_st8(ts + j0 + 8, lo);
+                    sum = rt_add2(sum, rt_weights(s, j0 < 32 ? fa : fb, use, ts + j0));
                 }
                 l = fmaf(l, corr, sum.x + sum.y);
                 sm.alpha[g & 3u][i] = corr;

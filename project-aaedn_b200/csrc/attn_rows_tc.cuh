@@ -150,11 +150,19 @@ __device__ __forceinline__ RtSeq rt_seq(const AttnRowsArgs& a, int s, int R)
     return q;
 }
 
-// Where a CTA starts (also what the joining kernel reads).
+// A tile costs its units and RT_TILE_COST more (its queries, the first and
+// last unit's latencies, its output): shares are equal in this measure, so a
+// share of many short tiles has fewer units. Measured per unit 1.5 us and per
+// tile 3 to 4 us: with no tile cost, the shares over short caches took 1.7
+// times as long as the average one.
+constexpr int RT_TILE_COST = 2;
+
+// Where a share starts (also what the joining kernel reads; the entry behind
+// the last share holds the end).
 struct RtStart
 {
     int s, h, t, u;            // sequence, K/V head, tile, unit in the tile
-    unsigned long long begin;  // first unit of the CTA's share
+    unsigned long long begin;  // the units before it
     unsigned long long total;  // units of the call
 };
 
@@ -172,67 +180,83 @@ __device__ __forceinline__ float* rt_slot(const AttnRowsArgs& a, int cta, int wh
                                     (size_t)(cta * 2 + which) * rt_slot_bytes<HDP>());
 }
 
-__device__ __forceinline__ unsigned long long rt_share(unsigned long long total, int cta, int grid)
-{
-    return total * (unsigned)cta / (unsigned)grid;
-}
-
-// The position of unit `at` (one warp; the result in every lane).
+// The start of share `share` of `shares` (one warp; the result in every lane).
 template <bool TREE>
-__device__ __noinline__ RtStart rt_locate(const AttnRowsArgs a, int R, int cta, int grid)
+__device__ __noinline__ RtStart rt_locate(const AttnRowsArgs a, int R, int share, int shares)
 {
     const int lane = threadIdx.x & 31;
-    auto units_of = [&](int s) -> unsigned long long {
+    // units and tiles of a sequence
+    auto size_of = [&](int s, unsigned long long& units, unsigned long long& tiles) {
+        units = tiles = 0;
         if (s >= a.n_seqs)
-            return 0;
+            return;
         const RtSeq q = rt_seq(a, s, R);
-        return q.n ? (unsigned long long)a.n_kv * rt_units_before(q, TREE, R, q.tiles) : 0;
+        if (!q.n)
+            return;
+        units = (unsigned long long)a.n_kv * rt_units_before(q, TREE, R, q.tiles);
+        tiles = (unsigned long long)a.n_kv * (unsigned)q.tiles;
     };
-    unsigned long long total = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
-        total += units_of(s0 + lane);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-    RtStart r{};
-    r.total = total;
-    r.begin = rt_share(total, cta, grid);
-    unsigned long long before = 0;
+    unsigned long long cost = 0, total = 0, un, ti;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
     {
-        const unsigned long long mine = units_of(s0 + lane);
-        unsigned long long incl = mine;
+        size_of(s0 + lane, un, ti);
+        total += un;
+        cost += un + RT_TILE_COST * ti;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        cost += __shfl_xor_sync(0xffffffffu, cost, o);
+    }
+    RtStart r{};
+    r.total = total;
+    r.begin = total; // the end, unless found below
+    const unsigned long long at = cost * (unsigned)share / (unsigned)shares;
+    unsigned long long cost0 = 0, units0 = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
+    {
+        size_of(s0 + lane, un, ti);
+        unsigned long long ui = un, ci = un + RT_TILE_COST * ti;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1)
         {
-            const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
+            const unsigned long long v = __shfl_up_sync(0xffffffffu, ui, o), w = __shfl_up_sync(0xffffffffu, ci, o);
             if (lane >= o)
-                incl += v;
+            {
+                ui += v;
+                ci += w;
+            }
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > r.begin);
+        const unsigned hit = __ballot_sync(0xffffffffu, cost0 + ci > at);
         if (hit)
         {
             const int l = __ffs(hit) - 1;
             r.s = s0 + l;
-            unsigned long long off = r.begin - before - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, mine, l));
+            const unsigned long long su = __shfl_sync(0xffffffffu, un, l), st = __shfl_sync(0xffffffffu, ti, l);
+            unsigned long long off = at - (cost0 + __shfl_sync(0xffffffffu, ci, l) - su - RT_TILE_COST * st);
+            r.begin = units0 + __shfl_sync(0xffffffffu, ui, l) - su;
             const RtSeq q = rt_seq(a, r.s, R);
-            const unsigned long long per = rt_units_before(q, TREE, R, q.tiles);
-            r.h = (int)(off / per);
-            off -= per * (unsigned)r.h;
-            int lo = 0, hi = q.tiles - 1; // the last tile with units_before(tile) <= off
+            const unsigned long long per = su / (unsigned)a.n_kv, pc = per + RT_TILE_COST * (unsigned)q.tiles;
+            r.h = (int)(off / pc);
+            off -= pc * (unsigned)r.h;
+            int lo = 0, hi = q.tiles - 1; // the last tile whose cost starts at or before off
             while (lo < hi)
             {
                 const int mid = (lo + hi + 1) >> 1;
-                if (rt_units_before(q, TREE, R, mid) <= off)
+                if (rt_units_before(q, TREE, R, mid) + (unsigned long long)RT_TILE_COST * mid <= off)
                     lo = mid;
                 else
                     hi = mid - 1;
             }
+            const unsigned long long before = rt_units_before(q, TREE, R, lo), in = off - before - (unsigned long long)RT_TILE_COST * lo;
             r.t = lo;
-            r.u = (int)(off - rt_units_before(q, TREE, R, lo));
+            r.u = in > RT_TILE_COST ? (int)(in - RT_TILE_COST) : 0; // the tile's own cost comes first
+            r.begin += per * (unsigned)r.h + before + (unsigned)r.u;
             break;
         }
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        units0 += __shfl_sync(0xffffffffu, ui, 31);
+        cost0 += __shfl_sync(0xffffffffu, ci, 31);
     }
     return r;
 }
@@ -438,24 +462,25 @@ __device__ __forceinline__ void rt_regs_dec()
 }
 
 // Waits for the phase with the given parity; false: another role gave up, or
-// 2^22 tries (of up to a microsecond each) ran out. No clock and no call, to
-// keep the many waits small.
+// about two seconds passed. The clock is read once in 256 tries. (A suspend
+// hint on the tries cost up to a microsecond of each wake-up.)
 __device__ __forceinline__ bool rt_wait(uint32_t bar, uint32_t parity, const volatile uint32_t* abort)
 {
-    for (uint32_t n = 0; n < (1u << 22); ++n)
+    uint64_t t0 = 0;
+    for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n)
     {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok)
-                     : "r"(bar), "r"(parity)
-                     : "memory");
-        if (ok)
-            return true;
         if (*abort)
             return false;
+        if ((n & 255u) == 255u)
+        {
+            const uint64_t t = globaltimer_ns();
+            if (t0 == 0)
+                t0 = t;
+            else if (t - t0 > RT_WAIT_LIMIT_NS)
+                return false;
+        }
     }
-    return false;
+    return true;
 }
 
 struct RtUnitInfo
@@ -470,7 +495,7 @@ struct RtShared
     uint64_t raw[8], conv[8], free_[8]; // per stage: copied, converted, read by the MMAs
     uint64_t s_full[2], p_full[2], o_full, o_empty, q_raw[4], q_full[2], q_empty[2], done;
     uint32_t tmem, abort;
-    RtStart start;
+    RtStart start, end;
     int stage_valid[8];
     alignas(16) uint32_t wmax[2][8];
     RtUnitInfo info[RT_INFO];
@@ -503,6 +528,39 @@ __device__ __forceinline__ void rt_mask16(float (&s)[16], uint32_t seen)
 #pragma unroll
     for (int j = 0; j < 16; ++j)
         s[j] = (seen >> j) & 1u ? s[j] : -INFINITY;
+}
+
+__device__ __forceinline__ float rt_max16(const float (&s)[16])
+{
+    float m0 = s[0], m1 = s[1];
+#pragma unroll
+    for (int j = 2; j < 16; j += 2)
+    {
+        m0 = fmaxf(m0, s[j]);
+        m1 = fmaxf(m1, s[j + 1]);
+    }
+    return fmaxf(m0, m1);
+}
+
+// Weights exp2(s f + use) of 16 scores into tensor memory at `t` (8 columns of
+// high and 8 of low parts); returns their sum (fp32, two halves).
+__device__ __forceinline__ float2 rt_weights(const float (&s)[16], float f, float use, uint32_t t)
+{
+    const float2 f2 = make_float2(f, f), use2 = make_float2(use, use);
+    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+    {
+        float2 x = fma2_rn(make_float2(s[2 * j], s[2 * j + 1]), f2, use2);
+        x.x = rt_exp2(x.x);
+        x.y = rt_exp2(x.y);
+        part[j & 1] = rt_add2(part[j & 1], x);
+        rt_split2(x.x, x.y, hi[j], lo[j]);
+    }
+    rt_st8(t, hi);
+    rt_st8(t + 8, lo);
+    return rt_add2(part[0], part[1]);
 }
 
 // Which of the 64 keys of a unit a row attends. limit: causal: the row's last
@@ -570,6 +628,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             reinterpret_cast<RtStart*>(a.workspace)[blockIdx.x] = st;
         }
     }
+    else if (warp == 3)
+    {
+        const RtStart en = rt_locate<TREE>(a, R, blockIdx.x + 1, gridDim.x);
+        if (lane == 0)
+        {
+            sm.end = en;
+            if (blockIdx.x + 1 == gridDim.x)
+                reinterpret_cast<RtStart*>(a.workspace)[gridDim.x] = en;
+        }
+    }
     else if (warp == 1)
     {
         if (lane == 0)
@@ -611,7 +679,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
     rt_fence_after();
     constexpr uint32_t tmem = 0u; // all columns are the CTA's
     const RtStart st0 = sm.start;
-    unsigned long long share = rt_share(st0.total, blockIdx.x + 1, gridDim.x) - st0.begin;
+    unsigned long long share = sm.end.begin - st0.begin;
     if (sm.tmem != tmem) // cannot be: nothing runs on other columns
     {
         share = 0;
@@ -805,48 +873,31 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     (seen & ((uint64_t)in.kbad[0] | (uint64_t)in.kbad[1] << 32)) != 0ull)
                     bad = true;
                 const bool all = __all_sync(0xffffffffu, seen == ~0ull);
-                // 16 keys at a time, twice: the largest score, then the weights
-                // (P takes the place of S: 8 columns of high, 8 of low parts)
-                float s[16], m0 = -INFINITY, m1 = -INFINITY;
+                // 16 keys at a time, twice: the largest score, then the weights (P takes
+                // the place of S). Rolled loops over tensor memory: with all 64
+                // scores in registers a unit alone is faster, the kernel 13 % slower
+                // (its roles' code no longer fits the instruction caches).
+                float s[16], top = -INFINITY;
 #pragma unroll 1
                 for (uint32_t j0 = 0; j0 < 64; j0 += 16)
                 {
                     rt_ld<16>(ts + j0, s);
                     if (!all)
                         rt_mask16(s, (uint32_t)(seen >> j0));
-#pragma unroll
-                    for (int j = 0; j < 16; j += 4)
-                    {
-                        m0 = fmaxf(m0, fmaxf(s[j], s[j + 1]));
-                        m1 = fmaxf(m1, fmaxf(s[j + 2], s[j + 3]));
-                    }
+                    top = fmaxf(top, rt_max16(s) * f);
                 }
-                const float noff = fminf(off, 14.0f - fmaxf(m0, m1) * f);
+                const float noff = fminf(off, 14.0f - top);
                 const float use = noff < INFINITY ? noff : 0.0f;
                 const float corr = rt_exp2(use - off); // 0 before the first key
                 off = noff;
                 float2 sum = make_float2(0.f, 0.f);
-                const float2 f2 = make_float2(f, f), use2 = make_float2(use, use);
 #pragma unroll 1
                 for (uint32_t j0 = 0; j0 < 64; j0 += 16)
                 {
                     rt_ld<16>(ts + j0, s);
                     if (!all)
                         rt_mask16(s, (uint32_t)(seen >> j0));
-                    uint32_t hi[8], lo[8];
-                    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                    {
-                        float2 x = fma2_rn(make_float2(s[2 * j], s[2 * j + 1]), f2, use2);
-                        x.x = rt_exp2(x.x);
-                        x.y = rt_exp2(x.y);
-                        part[j & 1] = rt_add2(part[j & 1], x);
-                        rt_split2(x.x, x.y, hi[j], lo[j]);
-                    }
-                    sum = rt_add2(sum, rt_add2(part[0], part[1]));
-                    rt_st8(ts + j0, hi);
-                    rt_st8(ts + j0 + 8, lo);
+                    sum = rt_add2(sum, rt_weights(s, f, use, ts + j0));
                 }
                 l = fmaf(l, corr, sum.x + sum.y);
                 sm.alpha[g & 3u][i] = corr;
@@ -1190,11 +1241,12 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
     const int c0 = blockIdx.x + 1, lane = threadIdx.x & 31;
     const RtStart* starts = reinterpret_cast<const RtStart*>(a.workspace);
     const RtStart st = starts[c0];
-    // the share of CTA c0 starts inside a tile, and no earlier one does
+    auto begin = [&](int c) { return starts[c].begin; };
+    // share c0 starts inside a tile, and no earlier one does
     if (st.u == 0 || st.begin >= st.total)
         return;
     const unsigned long long t0 = st.begin - (unsigned)st.u;
-    if (rt_share(st.total, c0 - 1, grid) > t0)
+    if (begin(c0 - 1) > t0)
         return;
     const int G = a.n_heads / a.n_kv, R = 128 / G, i2 = blockIdx.y * RJ_WARPS + (threadIdx.x >> 5);
     const int part = i2 >> 7, i = i2 & 127, ti = i / G; // CTA of the share, row of the CTA
@@ -1203,19 +1255,14 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
     if (ti >= R || r >= q.n)
         return;
     const unsigned long long t1 = t0 + (unsigned)((rt_keys(q, TREE, NC * R, st.t) + 63) / 64);
-    // the first share with a unit of the tile: the last one that starts at or before it and is not empty
-    int first = c0 - 1;
-    while (first > 0 && rt_share(st.total, first, grid) > t0)
-        --first;
-    while (rt_share(st.total, first + 1, grid) <= t0)
-        ++first;
+    const int first = c0 - 1; // starts at or before the tile and ends inside it
     // lane j takes the weights of share first + j, 32 at a time
     const float2 none = make_float2(0.0f, INFINITY);
     auto stat_of = [&](int c) -> float2 {
         if (c >= grid)
             return none;
-        const unsigned long long b = rt_share(st.total, c, grid);
-        if (b >= t1 || rt_share(st.total, c + 1, grid) == b)
+        const unsigned long long b = begin(c);
+        if (b >= t1 || begin(c + 1) == b)
             return none;
         return __ldcg(reinterpret_cast<const float2*>(rt_slot<HDP>(a, c * NC + part, b >= t0 ? 0 : 1) + 128 * HDP) + i);
     };
@@ -1225,7 +1272,7 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         while (last < hi)
         {
             const int mid = (last + hi + 1) >> 1;
-            if (rt_share(st.total, mid, grid) < t1)
+            if (begin(mid) < t1)
                 last = mid;
             else
                 hi = mid - 1;
@@ -1249,7 +1296,7 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         {
             const float wj = __shfl_sync(0xffffffffu, w, j);
             // an empty share (weight 0) has no sums: its slot is not read
-            const float* slot = rt_slot<HDP>(a, (c + j) * NC + part, j > 0 || c > first || rt_share(st.total, first, grid) >= t0 ? 0 : 1);
+            const float* slot = rt_slot<HDP>(a, (c + j) * NC + part, j > 0 || c > first || begin(first) >= t0 ? 0 : 1);
             const bool some = __shfl_sync(0xffffffffu, s.y, j) < INFINITY;
 #pragma unroll
             for (int d = 0; d < HDP / 32; ++d)
