@@ -20,12 +20,14 @@
 // bits.
 //
 // A row is a thread-block cluster of C CTAs, each with a slice of the
-// vocabulary in registers (one read of the logits). One pass makes a
-// histogram (count and mass) over 1024 equal steps of M - l; a search picks
-// the step that crosses its target, gathers that step's few tokens in the
-// first CTA, sorts them and scans their masses. A step with more tokens
-// than the list holds (ties, far outliers) is first narrowed by a radix
-// descent over (logit bits, id), 10 bits a pass.
+// vocabulary in shared memory (one read of the logits). One pass makes a
+// histogram of the masses over 1024 equal steps of M - l; a search picks the
+// step that crosses its target, gathers that step's few tokens in the first
+// CTA, sorts them and scans their masses. A step with more tokens than the
+// list holds (ties, far outliers) is narrowed by a radix descent over (logit
+// bits, id), 10 bits a pass. With top_k the first histogram only counts (one
+// shared-memory atomic a token in place of three, no exponential), and where
+// the tokens up to the k-th's step fit the list, one sort answers all.
 #include "common.cuh"
 
 #include "device_check.hpp"
@@ -40,6 +42,7 @@ namespace
 constexpr int SR_THREADS = 1024, SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = 1024; // one per thread
 constexpr int SR_LIST = 512;
+constexpr uint32_t SR_SLICE = 40000; // logits of a CTA in shared memory
 constexpr int SR_MASS_BITS = 45;
 
 struct SrShared
@@ -189,7 +192,6 @@ __device__ __forceinline__ void sr_clear(SrShared& s)
 
 __device__ __forceinline__ void sr_add(SrShared& s, int bin, uint64_t mass)
 {
-    atomicAdd(&s.cnt[bin], 1u);
     if (mass)
     {
         atomicAdd(&s.m0[bin], (uint32_t)(mass & 0x7FFF));
@@ -230,47 +232,83 @@ __device__ __forceinline__ void sr_collect(SrShared& s, uint32_t& c, uint64_t& m
     }
 }
 
-// C CTAs a row; E > 0: up to E logits of the slice per thread in registers,
-// E == 0: the slice is read again in every pass (from L2 after the first).
-template <int C, int E>
+// One token into the first CTA's list (what does not fit is counted only).
+template <int C>
+__device__ __forceinline__ void sr_append(SrShared& s, uint64_t key, uint64_t mass)
+{
+    if constexpr (C == 1)
+    {
+        const uint32_t at = atomicAdd(&s.n_list, 1u);
+        if (at < (uint32_t)SR_LIST)
+        {
+            s.lkey[at] = key;
+            s.lmass[at] = mass;
+        }
+    }
+    else
+    {
+        const uint32_t at = peer_add32(peer_addr(&s.n_list, 0), 1u);
+        if (at < (uint32_t)SR_LIST)
+        {
+            peer_st64(peer_addr(&s.lkey[at], 0), key);
+            peer_st64(peer_addr(&s.lmass[at], 0), mass);
+        }
+    }
+}
+
+// The list's first n tokens in order into skey / smass: a token's place is how
+// many keys are larger (keys are distinct). Two threads count for a token.
+__device__ __forceinline__ void sr_sort(SrShared& s, uint32_t n)
+{
+    static_assert(SR_THREADS == 2 * SR_LIST, "two threads a token");
+    const uint32_t i = threadIdx.x >> 1, part = threadIdx.x & 1;
+    uint32_t place = 0;
+    if (i < n)
+    {
+        const uint64_t key = s.lkey[i];
+#pragma unroll 4
+        for (uint32_t j = part; j < n; j += 2)
+            place += s.lkey[j] > key;
+    }
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    if (i < n && part == 0)
+    {
+        s.skey[place] = s.lkey[i];
+        s.smass[place] = s.lmass[i];
+    }
+    __syncthreads();
+}
+
+// C CTAs a row; RES: the slice's logits stay in shared memory, else every pass
+// reads them again (from L2 after the first).
+template <int C, bool RES>
 __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const SampleRowsArgs a)
 {
     extern __shared__ __align__(16) uint8_t sr_raw[];
     SrShared& s = *reinterpret_cast<SrShared*>(sr_raw);
+    float* slice = reinterpret_cast<float*>(sr_raw + sizeof(SrShared));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t row = blockIdx.x / C, rank = blockIdx.x % C;
     const uint32_t per = (a.vocab + C - 1) / C;
     const uint32_t v0 = rank * per, n_mine = v0 < a.vocab ? min(per, a.vocab - v0) : 0u;
     const float* src = a.logits + (size_t)row * a.ld + v0;
-    const float NANF = __uint_as_float(0x7FC00000u);
 
-    float e[E > 0 ? E : 1];
-    if constexpr (E > 0)
+    if constexpr (RES)
     {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-        {
-            const uint32_t j = (uint32_t)i * SR_THREADS + tid;
-            e[i] = j < n_mine ? __ldcs(src + j) : NANF;
-        }
+        // a thread reads back only what it wrote
+#pragma unroll 8
+        for (uint32_t j = tid; j < n_mine; j += SR_THREADS)
+            slice[j] = __ldcs(src + j);
     }
-    // fn(logit, id) for each of this thread's tokens that is not NaN
+    // fn(logit, id) for each of this thread's tokens that is not NaN. Rolled:
+    // unrolled over registers, the passes' code outgrew the instruction caches.
     auto each = [&](auto&& fn) {
-        if constexpr (E > 0)
+#pragma unroll 2
+        for (uint32_t j = tid; j < n_mine; j += SR_THREADS)
         {
-#pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (e[i] == e[i])
-                    fn(e[i], v0 + (uint32_t)i * SR_THREADS + tid);
-        }
-        else
-        {
-            for (uint32_t j = tid; j < n_mine; j += SR_THREADS)
-            {
-                const float l = src[j];
-                if (l == l)
-                    fn(l, v0 + j);
-            }
+            const float l = RES ? slice[j] : src[j];
+            if (l == l)
+                fn(l, v0 + j);
         }
     };
 
@@ -356,25 +394,109 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
     const float span = fminf(mx - mn, 40.0f * T);
     R.invw = span > 0.0f ? (float)SR_BINS / span : 0.0f;
 
-    // ---- count and mass of the 1024 steps of M - l, then their prefix sums
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const bool cut_k = k > 0 && (uint32_t)k < a.vocab;
+    const float tp = a.top_p ? a.top_p[row] : 1.0f;
+    const float uu = a.u[row];
     __syncthreads();
-    each([&](float l, uint32_t) { sr_add(s, sr_bin(l, R), sr_mass(l, R, s.tbl)); });
-    row_sync<C>();
     uint32_t c;
     uint64_t m;
-    sr_collect<C>(s, c, m);
-    sr_scan(c, m, s);
-    s.pc[tid] = c;
-    s.pm[tid] = m;
+    uint64_t key, W;
+    if (cut_k)
+    {
+        // ---- the step that holds the k-th token, by counts alone
+        each([&](float l, uint32_t) { atomicAdd(&s.cnt[sr_bin(l, R)], 1u); });
+        row_sync<C>();
+        sr_collect<C>(s, c, m);
+        const uint32_t own = c;
+        sr_scan(c, m, s);
+        if (c >= (uint32_t)k && c - own < (uint32_t)k)
+        {
+            s.pick = tid;
+            s.n_in = c;
+        }
+        if (tid == 0)
+        {
+            s.n_list = 0;
+            if (c == 0)
+                s.n_in = 0;
+        }
+        if (tid == SR_THREADS - 1 && c < (uint32_t)k) // fewer tokens than k (NaN logits): all of them
+        {
+            s.pick = SR_BINS - 1;
+            s.n_in = c;
+        }
+        row_sync<C>();
+        const int last = s.pick;
+        if (s.n_in <= (uint32_t)SR_LIST)
+        {
+            // everything that top_k can keep fits the list: one sort answers all
+            each([&](float l, uint32_t id) {
+                if (sr_bin(l, R) <= last)
+                    sr_append<C>(s, order_key(l, id), sr_mass(l, R, s.tbl));
+            });
+            row_sync<C>();
+            if (rank == 0)
+            {
+                const uint32_t n = min(s.n_list, (uint32_t)SR_LIST), kept = min(n, (uint32_t)k);
+                sr_sort(s, n);
+                uint32_t lc = 0;
+                uint64_t lm = tid < (int)kept ? s.smass[tid] : 0ull;
+                const uint64_t own_m = lm;
+                sr_scan(lc, lm, s);
+                if (tid < (int)kept)
+                    s.lmass[tid] = lm; // cumulative
+                __syncthreads();
+                // first i with cum[i] >= target
+                auto cross = [&](double target) {
+                    const bool in = tid < (int)kept && (double)lm >= target;
+                    const bool before = tid < (int)kept && tid > 0 && (double)(lm - own_m) >= target;
+                    if (in && !before)
+                        s.pick = tid;
+                    __syncthreads();
+                    const int at = s.pick;
+                    __syncthreads();
+                    return at;
+                };
+                W = kept ? s.lmass[kept - 1] : 0ull;
+                if (tp < 1.0f)
+                    W = s.lmass[cross((double)tp * (double)W)];
+                const int at = cross(uu > 0.0f ? fmin((double)uu, 1.0) * (double)W : 0.0);
+                if (tid == 0)
+                    a.tokens[row] = 0xFFFFFFFFu - (uint32_t)(s.skey[at] & 0xFFFFFFFFu);
+            }
+            return; // no CTA reads another's shared memory after the last barrier
+        }
+        // more tokens than that: the masses of the steps up to the cut
+        sr_clear(s);
+        __syncthreads();
+        each([&](float l, uint32_t) {
+            const int b = sr_bin(l, R);
+            if (b <= last)
+                sr_add(s, b, sr_mass(l, R, s.tbl));
+        });
+        s.pc[tid] = c;
+    }
+    else
+        // ---- the masses of the 1024 steps of M - l
+        each([&](float l, uint32_t) { sr_add(s, sr_bin(l, R), sr_mass(l, R, s.tbl)); });
+    row_sync<C>();
+    {
+        uint32_t unused;
+        sr_collect<C>(s, unused, m);
+        unused = 0;
+        sr_scan(unused, m, s);
+    }
+    s.pm[tid] = m; // cumulative
     row_sync<C>(); // the histograms are free again
 
     // The first token whose cumulative count (by_count) or mass reaches the
     // target: its order key and the mass up to and including it.
     auto search = [&](bool by_count, uint32_t k, double target, uint64_t& key_out, uint64_t& mass_out) {
-        // one thread a step; hit: this step crosses the target
-        auto pick_step = [&](uint32_t c_incl, uint64_t m_incl, uint32_t c_excl, uint64_t m_excl) {
-            const bool in = by_count ? c_incl >= k : (c_incl > 0 && (double)m_incl >= target);
-            const bool before = by_count ? c_excl >= k : (c_excl > 0 && (double)m_excl >= target);
+        // one thread a step (or digit); hit: it crosses the target
+        auto pick_step = [&](uint32_t c_incl, uint64_t m_incl, uint32_t c_excl, uint64_t m_excl, bool first) {
+            const bool in = by_count ? c_incl >= k : (double)m_incl >= target;
+            const bool before = !first && (by_count ? c_excl >= k : (double)m_excl >= target);
             if (in && !before)
             {
                 s.pick = tid;
@@ -383,26 +505,46 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
                 s.n_in = c_incl - c_excl;
             }
         };
-        pick_step(s.pc[tid], s.pm[tid], tid ? s.pc[tid - 1] : 0u, tid ? s.pm[tid - 1] : 0ull);
+        // the step of the largest logit is the first and never empty, so a target of 0 ends there
+        pick_step(by_count ? s.pc[tid] : 0u, s.pm[tid], by_count && tid ? s.pc[tid - 1] : 0u, tid ? s.pm[tid - 1] : 0ull,
+                  tid == 0);
         if (tid == 0)
             s.n_list = 0;
         __syncthreads();
         const int step = s.pick;
-        uint32_t above_c = s.above_c, n_in = s.n_in;
+        uint32_t above_c = s.above_c;
         uint64_t above_m = s.above_m;
         uint64_t prefix = 0;
         int shift = 64; // the key bits from here up are fixed to prefix
+        auto mine = [&](uint64_t key) { return shift == 64 || (key >> shift) == (prefix >> shift); };
         row_sync<C>(); // n_list is zero in every CTA
-        while (n_in > (uint32_t)SR_LIST && shift > 0)
+        while (true)
         {
-            // narrow the step: the next 10 bits of the order key
+            // gather the step's tokens in the first CTA
+            each([&](float l, uint32_t id) {
+                if (sr_bin(l, R) == step)
+                {
+                    const uint64_t key = order_key(l, id);
+                    if (mine(key))
+                        sr_append<C>(s, key, sr_mass(l, R, s.tbl));
+                }
+            });
+            row_sync<C>();
+            const uint32_t n = C == 1 ? s.n_list : peer_ld32(peer_addr(&s.n_list, 0));
+            if (n <= (uint32_t)SR_LIST || shift == 0)
+                break;
+            // too many: narrow the step by the next 10 bits of the order key
             const int nshift = shift > 10 ? shift - 10 : 0;
             sr_clear(s);
             __syncthreads();
             each([&](float l, uint32_t id) {
                 const uint64_t key = order_key(l, id);
-                if (sr_bin(l, R) == step && (shift == 64 || (key >> shift) == (prefix >> shift)))
-                    sr_add(s, SR_BINS - 1 - (int)((key >> nshift) & ((1u << (shift - nshift)) - 1u)), sr_mass(l, R, s.tbl));
+                if (sr_bin(l, R) == step && mine(key))
+                {
+                    const int d = SR_BINS - 1 - (int)((key >> nshift) & ((1u << (shift - nshift)) - 1u));
+                    atomicAdd(&s.cnt[d], 1u);
+                    sr_add(s, d, sr_mass(l, R, s.tbl));
+                }
             });
             row_sync<C>();
             uint32_t dc;
@@ -411,58 +553,22 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
             const uint32_t own_c = dc;
             const uint64_t own_m = dm;
             sr_scan(dc, dm, s);
-            pick_step(above_c + dc, above_m + dm, above_c + dc - own_c, above_m + dm - own_m);
+            // an empty digit cannot be the one (a target of 0 ends at the first token)
+            if (own_c)
+                pick_step(above_c + dc, above_m + dm, above_c + dc - own_c, above_m + dm - own_m, dc == own_c);
+            if (tid == 0)
+                s.n_list = 0;
             __syncthreads();
             prefix |= (uint64_t)(SR_BINS - 1 - s.pick) << nshift;
             shift = nshift;
             above_c = s.above_c;
             above_m = s.above_m;
-            n_in = s.n_in;
             row_sync<C>();
         }
-        // gather the step's tokens in the first CTA
-        each([&](float l, uint32_t id) {
-            if (sr_bin(l, R) == step)
-            {
-                const uint64_t key = order_key(l, id);
-                if (shift == 64 || (key >> shift) == (prefix >> shift))
-                {
-                    const uint64_t mass = sr_mass(l, R, s.tbl);
-                    if constexpr (C == 1)
-                    {
-                        const uint32_t at = atomicAdd(&s.n_list, 1u);
-                        if (at < (uint32_t)SR_LIST)
-                        {
-                            s.lkey[at] = key;
-                            s.lmass[at] = mass;
-                        }
-                    }
-                    else
-                    {
-                        const uint32_t at = peer_add32(peer_addr(&s.n_list, 0), 1u);
-                        if (at < (uint32_t)SR_LIST)
-                        {
-                            peer_st64(peer_addr(&s.lkey[at], 0), key);
-                            peer_st64(peer_addr(&s.lmass[at], 0), mass);
-                        }
-                    }
-                }
-            }
-        });
-        row_sync<C>();
         if (rank == 0)
         {
             const uint32_t n = min(s.n_list, (uint32_t)SR_LIST);
-            if (tid < (int)n) // a token's place: how many keys are larger (keys are distinct)
-            {
-                const uint64_t key = s.lkey[tid];
-                uint32_t place = 0;
-                for (uint32_t j = 0; j < n; ++j)
-                    place += s.lkey[j] > key;
-                s.skey[place] = key;
-                s.smass[place] = s.lmass[tid];
-            }
-            __syncthreads();
+            sr_sort(s, n);
             uint32_t lc = tid < (int)n ? 1u : 0u;
             uint64_t lm = tid < (int)n ? s.smass[tid] : 0ull;
             const uint64_t own = lm;
@@ -494,27 +600,24 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         mass_out = s.found_mass;
     };
 
-    uint64_t key, W = s.pm[SR_BINS - 1];
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && (uint32_t)k < s.pc[SR_BINS - 1])
+    W = s.pm[SR_BINS - 1];
+    if (cut_k && (uint32_t)k < s.pc[SR_BINS - 1])
         search(true, (uint32_t)k, 0.0, key, W);
-    const float tp = a.top_p ? a.top_p[row] : 1.0f;
     if (tp < 1.0f)
         search(false, 0, (double)tp * (double)W, key, W);
-    const float uu = a.u[row];
     search(false, 0, uu > 0.0f ? fmin((double)uu, 1.0) * (double)W : 0.0, key, W);
     if (rank == 0 && tid == 0)
         a.tokens[row] = 0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFu);
     row_sync<C>();
 }
 
-template <int C, int E>
+template <int C, bool RES>
 int sr_launch(const SampleRowsArgs& a, cudaStream_t st)
 {
     static PerDeviceOnce attrs;
     const int arc = attrs.run([]() -> int {
-        AAEDN_CUDA_TRY(cudaFuncSetAttribute(sample_rows_kernel<C, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            (int)sizeof(SrShared)));
+        AAEDN_CUDA_TRY(cudaFuncSetAttribute(sample_rows_kernel<C, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)(sizeof(SrShared) + (RES ? SR_SLICE * 4 : 0))));
         return AAEDN_OK;
     });
     if (arc)
@@ -522,7 +625,7 @@ int sr_launch(const SampleRowsArgs& a, cudaStream_t st)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.rows * C);
     cfg.blockDim = dim3(SR_THREADS);
-    cfg.dynamicSmemBytes = sizeof(SrShared);
+    cfg.dynamicSmemBytes = sizeof(SrShared) + (RES ? (size_t)(a.vocab + C - 1) / C * 4 : 0);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -531,43 +634,30 @@ int sr_launch(const SampleRowsArgs& a, cudaStream_t st)
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_rows_kernel<C, E>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_rows_kernel<C, RES>, a);
     if (e != cudaSuccess)
         return set_error(AAEDN_ECUDA, "launch of sample_rows_kernel failed: %s", cudaGetErrorString(e));
     count_launch();
     return AAEDN_OK;
 }
 
-template <int C>
-int sr_launch_e(const SampleRowsArgs& a, cudaStream_t st)
-{
-    const uint32_t per = (a.vocab + C - 1) / C;
-    if (per <= 8u * SR_THREADS)
-        return sr_launch<C, 8>(a, st);
-    if (per <= 16u * SR_THREADS)
-        return sr_launch<C, 16>(a, st);
-    if (per <= 32u * SR_THREADS)
-        return sr_launch<C, 32>(a, st);
-    return sr_launch<C, 0>(a, st);
-}
-
 } // namespace
 
 int sample_rows(const SampleRowsArgs& a, cudaStream_t st)
 {
-    // the fewest CTAs a row whose registers hold it (32 logits a thread),
-    // then more while the rows leave SMs idle and a CTA has over 2048 tokens
+    // the fewest CTAs a row whose shared memory holds it, then more while the
+    // rows leave SMs idle and a CTA has over 2048 tokens
     int C = 1;
-    while (C < 8 && (a.vocab + C - 1) / C > 32u * SR_THREADS)
+    while (C < 8 && (a.vocab + C - 1) / C > SR_SLICE)
         C *= 2;
     while (C < 8 && (size_t)a.rows * C * 2 <= (size_t)sm_count() && (a.vocab + C - 1) / C > 2048)
         C *= 2;
     switch (C)
     {
-    case 1: return sr_launch_e<1>(a, st);
-    case 2: return sr_launch_e<2>(a, st);
-    case 4: return sr_launch_e<4>(a, st);
-    default: return sr_launch_e<8>(a, st);
+    case 1: return sr_launch<1, true>(a, st);
+    case 2: return sr_launch<2, true>(a, st);
+    case 4: return sr_launch<4, true>(a, st);
+    default: return (a.vocab + 7) / 8 <= SR_SLICE ? sr_launch<8, true>(a, st) : sr_launch<8, false>(a, st);
     }
 }
 
