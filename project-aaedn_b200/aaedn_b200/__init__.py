@@ -405,8 +405,10 @@ def tree_masks(parents):
 
 def _arrays(d_arrays):
     """A host array of device pointers (pass one made earlier as it is)."""
-    if isinstance(d_arrays, ctypes.Array):
-        return d_arrays
+    if isinstance(d_arrays, ctypes.Array) or not len(d_arrays):
+        return d_arrays or (_vp * 0)()
+    if hasattr(d_arrays[0], "data_ptr"):
+        return (_vp * len(d_arrays))(*[a.data_ptr() for a in d_arrays])
     return (_vp * len(d_arrays))(*[_p(a) for a in d_arrays])
 
 

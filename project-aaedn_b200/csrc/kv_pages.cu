@@ -1,6 +1,10 @@
 // kv_pages.cu — copies of whole cache pages and the compaction of a
 // sequence's last slots, in every layer's K and V with one launch.
+#include <cuda.h>
+#include <cudaTypedefs.h> // PFN_cuMemGetAddressRange
+
 #include <climits>
+#include <mutex>
 
 #include "common.cuh"
 
@@ -163,6 +167,21 @@ int kv_compact(float* const* arrays, size_t n_arrays, const KvCompactArgs& a, cu
 
 using namespace aaedn_dev;
 
+// cuMemGetAddressRange of the driver, or null.
+static PFN_cuMemGetAddressRange_v3020 range_fn()
+{
+    static PFN_cuMemGetAddressRange_v3020 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, []() {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuMemGetAddressRange", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuMemGetAddressRange_v3020>(p);
+    });
+    return fn;
+}
+
 static int check_arrays(const char* fn, float* const* h_arrays, size_t n_arrays, uint32_t n_pages)
 {
     if (!h_arrays)
@@ -171,9 +190,25 @@ static int check_arrays(const char* fn, float* const* h_arrays, size_t n_arrays,
         return set_error(AAEDN_EINVAL, "%s: at most 4096 arrays (%zu)", fn, n_arrays);
     if (n_pages == 0 || n_pages > (uint32_t)INT_MAX)
         return set_error(AAEDN_EINVAL, "%s: n_pages %u", fn, n_pages);
+    // pools are mostly parts of one allocation: its extent, asked for once,
+    // vouches for the others in it (a query each took longer than the copies)
+    uintptr_t lo = 0, hi = 0;
+    const PFN_cuMemGetAddressRange_v3020 range = range_fn();
     for (size_t i = 0; i < n_arrays; ++i)
+    {
+        const uintptr_t p = reinterpret_cast<uintptr_t>(h_arrays[i]);
+        if (p >= lo && p < hi && (p & 15) == 0)
+            continue;
         if (int rc = check_device_ptr(fn, h_arrays[i], "an array", 16))
             return rc;
+        CUdeviceptr base = 0;
+        size_t size = 0;
+        if (range && range(&base, &size, (CUdeviceptr)p) == CUDA_SUCCESS)
+        {
+            lo = (uintptr_t)base;
+            hi = lo + size;
+        }
+    }
     return AAEDN_OK;
 }
 
