@@ -1241,12 +1241,13 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
     const int c0 = blockIdx.x + 1, lane = threadIdx.x & 31;
     const RtStart* starts = reinterpret_cast<const RtStart*>(a.workspace);
     const RtStart st = starts[c0];
-    auto begin = [&](int c) { return starts[c].begin; };
     // share c0 starts inside a tile, and no earlier one does
     if (st.u == 0 || st.begin >= st.total)
         return;
     const unsigned long long t0 = st.begin - (unsigned)st.u;
-    if (begin(c0 - 1) > t0)
+    const int first = c0 - 1; // starts at or before the tile and ends inside it
+    const unsigned long long begin0 = starts[first].begin;
+    if (begin0 > t0)
         return;
     const int G = a.n_heads / a.n_kv, R = 128 / G, i2 = blockIdx.y * RJ_WARPS + (threadIdx.x >> 5);
     const int part = i2 >> 7, i = i2 & 127, ti = i / G; // CTA of the share, row of the CTA
@@ -1255,53 +1256,56 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
     if (ti >= R || r >= q.n)
         return;
     const unsigned long long t1 = t0 + (unsigned)((rt_keys(q, TREE, NC * R, st.t) + 63) / 64);
-    const int first = c0 - 1; // starts at or before the tile and ends inside it
-    // lane j takes the weights of share first + j, 32 at a time
-    const float2 none = make_float2(0.0f, INFINITY);
-    auto stat_of = [&](int c) -> float2 {
-        if (c >= grid)
-            return none;
-        const unsigned long long b = begin(c);
-        if (b >= t1 || begin(c + 1) == b)
-            return none;
-        return __ldcg(reinterpret_cast<const float2*>(rt_slot<HDP>(a, c * NC + part, b >= t0 ? 0 : 1) + 128 * HDP) + i);
+    // lane j takes the sum and offset of share c + j, 32 shares at a time; a
+    // share without units of the tile has none
+    auto stat_of = [&](int c, bool& more) -> float2 {
+        float2 v = make_float2(0.0f, INFINITY);
+        const int k = c + lane;
+        const unsigned long long b = k < grid ? starts[k].begin : t1, e = k < grid ? starts[k + 1].begin : t1;
+        if (b < t1 && b < e)
+            v = __ldcg(reinterpret_cast<const float2*>(rt_slot<HDP>(a, k * NC + part, b >= t0 ? 0 : 1) + 128 * HDP) + i);
+        more = __all_sync(0xffffffffu, b < t1);
+        return v;
     };
-    int last = first; // the last share with a unit of the tile
-    {
-        int hi = grid - 1;
-        while (last < hi)
-        {
-            const int mid = (last + hi + 1) >> 1;
-            if (begin(mid) < t1)
-                last = mid;
-            else
-                hi = mid - 1;
-        }
-    }
-    float off = INFINITY;
-    for (int c = first; c <= last; c += 32)
-        off = fminf(off, -warp_max(-stat_of(c + lane).y));
+    bool more;
+    float2 s = stat_of(first, more);
+    float off = -warp_max(-s.y);
+    for (int c = first + 32; more; c += 32)
+        off = fminf(off, -warp_max(-stat_of(c, more).y));
     float l = 0.0f, acc[HDP / 32];
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
         acc[d] = 0.0f;
-    for (int c = first; c <= last; c += 32)
+    more = true;
+    for (int c = first; more; c += 32)
     {
-        const float2 s = stat_of(c + lane);
+        s = stat_of(c, more);
         const float w = s.y < INFINITY ? rt_exp2(off - s.y) : 0.0f;
         l += warp_sum(s.x * w);
-        const int n = min(32, last + 1 - c);
-#pragma unroll 4
-        for (int j = 0; j < n; ++j)
+        unsigned has = __ballot_sync(0xffffffffu, s.y < INFINITY);
+        // in order, four shares' sums loaded before the first is used
+        while (has)
         {
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            // an empty share (weight 0) has no sums: its slot is not read
-            const float* slot = rt_slot<HDP>(a, (c + j) * NC + part, j > 0 || c > first || begin(first) >= t0 ? 0 : 1);
-            const bool some = __shfl_sync(0xffffffffu, s.y, j) < INFINITY;
+            float v[4][HDP / 32], wj[4];
 #pragma unroll
-            for (int d = 0; d < HDP / 32; ++d)
-                if (some)
-                    acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), wj, acc[d]);
+            for (int k = 0; k < 4; ++k)
+            {
+                const int j = has ? __ffs(has) - 1 : -1;
+                has &= has - 1;
+                wj[k] = __shfl_sync(0xffffffffu, w, j < 0 ? 0 : j);
+                // the first share has the tile as its last item unless it starts with it
+                const float* slot = rt_slot<HDP>(a, (c + j) * NC + part, c + j > first || begin0 >= t0 ? 0 : 1);
+#pragma unroll
+                for (int d = 0; d < HDP / 32; ++d)
+                    v[k][d] = j < 0 ? 0.0f : __ldcg(slot + (size_t)i * HDP + d * 32 + lane);
+                if (j < 0)
+                    wj[k] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int d = 0; d < HDP / 32; ++d)
+                    acc[d] = fmaf(v[k][d], wj[k], acc[d]);
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
