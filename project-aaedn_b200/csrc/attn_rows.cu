@@ -58,13 +58,14 @@ namespace aaedn_dev
 {
 
 // ---------------------------------------------------------------------------
-// One warp per (packed row, query head), every head_dim (a multiple of 4, at
-// most 256). Keys come 32 at a time: lane j scores key s0 + j against q (in
-// shared memory), the softmax is carried online (running max and sum), then
-// the lanes take the head dims and add the keys' weighted V rows. fp32
-// throughout; a key that the row may not attend is never read, so what such
-// a slot holds (NaN, an unused page) has no effect. A row with no key gives
-// zeros.
+// One warp per (packed row, query head), for head_dim 129..256. Keys come 32
+// at a time: lane j scores key s0 + j against q (in shared memory), the softmax
+// is carried online (running max and sum), then the lanes take the head dims
+// and add the keys' weighted V rows. fp32 throughout; a key that the row may
+// not attend is never read, so what such a slot holds (NaN, an unused page) has
+// no effect. A row with no key gives zeros. Bound by its own loads: every row
+// reads its keys for itself, from L2 (1077 tokens, 16 heads of 256 dims: 2.9
+// ms).
 // ---------------------------------------------------------------------------
 constexpr int RW_WARPS = 4;
 
@@ -171,8 +172,8 @@ int attn_rows_init()
     static PerDeviceOnce once;
     return once.run([]() -> int {
         int rc;
-        if ((rc = rows_tc_attrs(attn_rows_tc_kernel<64, false>, RtCfg<64>::SMEM)) ||
-            (rc = rows_tc_attrs(attn_rows_tc_kernel<64, true>, RtCfg<64>::SMEM)) ||
+        if ((rc = rows_tc_attrs(attn_rows_tc_kernel<false>, RT_SMEM)) ||
+            (rc = rows_tc_attrs(attn_rows_tc_kernel<true>, RT_SMEM)) ||
             (rc = rows_tc_attrs(attn_rows_pair_kernel<false>, RP_SMEM)))
             return rc;
         return rows_tc_attrs(attn_rows_pair_kernel<true>, RP_SMEM);
@@ -272,18 +273,27 @@ static int rows_pair_launch(const AttnRowsArgs& a, cudaStream_t st)
     return rows_join<RP_HDP, TREE, 2>(a, pairs, st);
 }
 
-template <int HDP, bool TREE>
+template <bool TREE>
 static int rows_tc_launch(const AttnRowsArgs& a, cudaStream_t st)
 {
     unsigned* err;
     if (int rc = rows_err_word(a, &err))
         return rc;
-    const int grid = rows_grid<HDP>();
-    attn_rows_tc_kernel<HDP, TREE><<<grid, RT_THREADS, RtCfg<HDP>::SMEM, st>>>(a, err);
+    const int grid = rows_grid<RT_HDP>();
+    attn_rows_tc_kernel<TREE><<<grid, RT_THREADS, RT_SMEM, st>>>(a, err);
     AAEDN_LAUNCH_CHECK("attn_rows_tc_kernel");
-    return rows_join<HDP, TREE, 1>(a, grid, st);
+    return rows_join<RT_HDP, TREE, 1>(a, grid, st);
 }
 
+// The kernel by head_dim. Up to 64 one SM a tile: the pair's stages are 128
+// dims wide, and half of each MMA would be padding (prompt of 2048 tokens 123
+// us, by the pairs 131; a tree of 16 over 4001 tokens 26, by the pairs 34).
+// 65..128 the pairs (a prompt of 4096 tokens, 64 heads over 8: 924 us when they
+// came, by single SMs 1053; eight sequences of 4120 tokens 259 and 274).
+// Above, a tile's operands do not fit one SM's tensor memory beside its sums:
+// one warp a row (on prompts 70 to 90 times slower where both can run: 13.6
+// against 0.15 ms; only calls of a few rows over short caches lose nothing by
+// it: 5 rows without a cache 16 us, by the pairs 20).
 int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
 {
     if (a.head_dim <= 128)
@@ -291,7 +301,7 @@ int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
         if (int rc = attn_rows_init())
             return rc;
         if (a.head_dim <= 64)
-            return a.mask ? rows_tc_launch<64, true>(a, st) : rows_tc_launch<64, false>(a, st);
+            return a.mask ? rows_tc_launch<true>(a, st) : rows_tc_launch<false>(a, st);
         return a.mask ? rows_pair_launch<true>(a, st) : rows_pair_launch<false>(a, st);
     }
     const dim3 grid((unsigned)((a.rows + RW_WARPS - 1) / RW_WARPS), (unsigned)a.n_heads);

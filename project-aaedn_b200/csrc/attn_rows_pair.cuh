@@ -15,6 +15,21 @@
 //
 // The first CTA's warp 1 issues the MMAs of both; its barriers count the
 // arrivals of both CTAs, and its commits arrive on both CTAs' barriers.
+//
+// On a B200: one prompt of 4096 tokens, 64 query heads over 8, 800 us (three
+// MMAs of full rate a product would be 490, one 163); eight sequences of 4120
+// new tokens in all, 32 heads over 8, 196 us; 2048 tokens, 32 heads, 147 us; a
+// tree of 16 nodes over 4001 cached tokens, 32 heads over 8, 34 us; sixteen
+// trees of 1 to 63 nodes over 0 to 4032, 64 heads, 134 us. A unit takes about
+// 3000 clocks, its MMAs 1536: P V waits for the weights of both CTAs, the
+// output sums for P V, the next P V for them, and softmax and each conversion,
+// one warp a scheduler, take about 2500 clocks of latencies a unit themselves
+// (the ragged case: tensor pipe 41 % active, issue slots 49 %, HBM 13 %). With all of that arithmetic cut out the
+// handshakes and MMAs alone take 573 us of the 800. Tried and slower: two units
+// as one group through softmax, P V and sums (844 us: the conversions spill),
+// the maximum kept from earlier units instead of a first pass over the scores
+// (836), 64 scores in registers (900), one more pair of score buffers in the
+// place of the second Q buffer (equal).
 #pragma once
 
 #include <cuda.h> // CUtensorMap
@@ -27,6 +42,7 @@ namespace aaedn_dev
 constexpr int RP_HDP = 128, RP_NS = 4;   // stages of K, and of V
 constexpr uint32_t RP_STAGE = 16384;     // 32 keys x 128 dims, or 64 keys x 64 dims, of 4 bytes
 constexpr uint32_t RP_Q_ROW = RP_HDP * 4u + 16u;
+constexpr uint32_t RP_T_QLO = 64; // Q's low parts behind its high parts, in tensor memory columns
 constexpr size_t RP_SMEM = 2 * RP_NS * (size_t)RP_STAGE + 128 * RP_Q_ROW + 1024; // + alignment slack
 
 // What a CTA's converting warps say of their part of a unit; the other CTA's
@@ -303,7 +319,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
 #pragma unroll 1
                         for (uint32_t p = 0; p < 3; ++p) // q_hi k_lo, q_lo k_hi, q_hi k_hi
                         {
-                            const uint32_t q = RT_T_Q + qb * 128u + (p == 1 ? RT_T_QLO : 0u), k = k_hi + (p == 0 ? 512u : 0u);
+                            const uint32_t q = RT_T_Q + qb * 128u + (p == 1 ? RP_T_QLO : 0u), k = k_hi + (p == 0 ? 512u : 0u);
 #pragma unroll
                             for (uint32_t n = 0; n < HDP / 16; ++n)
                                 rp_mma(d, q + n * 8u, k + (n >> 2) * 256u + (n & 3u) * 2u, RT_DESC_HI, id_qk, p | n);
@@ -753,7 +769,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                     rt_split2(__uint_as_float(x.z) * q_up, __uint_as_float(x.w) * q_up, hi[2 * d + 1], lo[2 * d + 1]);
                 }
                 rt_st8(tmem + lanes + RT_T_Q + qb * 128u + d0 / 2, hi);
-                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + RT_T_QLO + d0 / 2, lo);
+                rt_st8(tmem + lanes + RT_T_Q + qb * 128u + RP_T_QLO + d0 / 2, lo);
             }
             rt_wait_st();
             rt_fence_before();
