@@ -277,9 +277,9 @@ int aaedn_cu_kv_copy_pages(float* const* h_arrays, size_t n_arrays, size_t page_
  * 1] - d_keep_start[s], the row of slot d_base[s] + i becomes what slot
  * d_base[s] + d_keep[d_keep_start[s] + i] held, in each of the n_arrays pools
  * ([n_pages][n_kv_heads][64][head_dim]). Each sequence's keep list is
- * strictly ascending from 0 up, n_keep entries in all (the length of d_keep); the sequences' slots lie in different pages
- * or do not overlap. Entries with a slot outside the table or a page outside
- * the pool are skipped. */
+ * strictly ascending from 0 up, n_keep entries in all (the length of d_keep);
+ * the sequences' slots lie in different pages or do not overlap. Entries with
+ * a slot outside the table or a page outside the pool are skipped. */
 int aaedn_cu_kv_compact(float* const* h_arrays, size_t n_arrays, uint32_t n_pages, uint32_t n_kv_heads,
                         uint32_t head_dim, const int32_t* d_page_table, size_t pt_stride, const int32_t* d_base,
                         const int32_t* d_keep, const int32_t* d_keep_start, size_t n_seqs, size_t n_keep,

@@ -211,6 +211,159 @@ def test_index_arrays_that_make_no_sense_stay_in_bounds():
         ab.device_sync()
 
 
+@pytest.mark.parametrize("H,KV,hd", [(64, 1, 16), (33, 1, 128), (64, 1, 192), (45, 15, 68)])
+def test_any_number_of_heads_on_a_kv_head(H, KV, hd):
+    c = ref.Case(H, KV, hd, [5, 1, 17], [70, 0, 3], seed=24)
+    _check(c, "packed", _call(c, "packed"))
+
+
+@pytest.mark.parametrize("hd", [32, 128, 160])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_scales(hd, scale):
+    c = ref.Case(4, 2, hd, [70, 3], [5, 80], seed=25)
+    c.scale = scale
+    _check(c, "packed", _call(c, "packed"))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 160])
+def test_trees_of_many_units(hd):
+    """256 nodes behind prefixes that end inside a page, at its end and nowhere."""
+    c = ref.Case(4, 2, hd, [256, 200, 129], [37, 64, 0], seed=26)
+    rng = np.random.default_rng(6)
+    masks = np.concatenate([ref.masks_of(ref.random_parents(rng, n), 4) for n in (256, 200, 129)])
+    _check(c, "tree", _call(c, "tree", masks, 4), masks)
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+def test_thousands_of_sequences(hd):
+    rng = np.random.default_rng(8)
+    rows = [int(x) for x in rng.integers(0, 3, 2500)]
+    past = [int(x) for x in rng.integers(0, 20, 2500)]
+    c = ref.Case(2, 1, hd, rows, past, seed=27)
+    _check(c, "packed", _call(c, "packed"))
+
+
+class _Bound:
+    """A call's device buffers, for running it many times."""
+
+    def __init__(self, c):
+        self.c = c
+        self.q, k, v, table = dev(c.q), dev(c.k), dev(c.v), dev(c.table)
+        self.start, self.past = dev(c.start), dev(np.array(c.past, np.int32))
+        self.cache = ab.KvCache(k, v, table, c.stride, c.n_pages, c.KV, c.hd)
+        self.out, self.ws = empty_f32(c.T * c.H * c.hd), _workspace()
+
+    def run(self, stream):
+        c = self.c
+        ab.attention_packed(self.q, self.cache, self.start, self.past, len(c.past), c.T, c.H, c.scale, self.out, self.ws,
+                            stream=stream)
+
+    def check(self):
+        c = self.c
+        want, tol = ref.attention("packed", c.q, c.k, c.v, c.table, c.start, c.past, c.H, c.scale)
+        assert np.all(np.abs(host(self.out).reshape(c.T, -1) - want) <= tol)
+
+
+def _bound_pair():
+    return (_Bound(ref.Case(8, 2, 128, [150, 9], [3, 500], seed=28)), _Bound(ref.Case(6, 6, 48, [200, 31], [0, 100], seed=29)),
+            _Bound(ref.Case(8, 2, 128, [90, 1], [64, 1000], seed=30)))
+
+
+def test_calls_at_once_on_several_streams():
+    import torch
+    calls = _bound_pair()
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for b, st in zip(calls, streams):
+            b.run(st.cuda_stream)
+    ab.device_sync()
+    for b in calls:
+        b.check()
+
+
+def test_captured_calls_at_once():
+    """Graphs with a workspace each, replayed on streams of their own."""
+    import torch
+    calls = _bound_pair()
+    streams = [torch.cuda.Stream() for _ in calls]
+    graphs = []
+    torch.cuda.synchronize()
+    for b, st in zip(calls, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(st):
+            g.capture_begin()
+            b.run(st.cuda_stream)
+            b.run(st.cuda_stream)  # twice on one workspace, one behind the other
+            g.capture_end()
+        graphs.append(g)
+    for _ in range(6):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    ab.device_sync()
+    for b in calls:
+        b.check()
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = {paths!r}
+import numpy as np, torch
+import aaedn_b200 as ab, batched_ops_ref as ref
+from gpu_util import dev, host
+what = sys.argv[1]
+st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+s = st.cuda_stream
+if what.startswith("attention"):
+    c = ref.Case(4, 2, int(what[9:]), [70, 3], [5, 200], seed=31)
+    q, cache = dev(c.q), ab.KvCache(dev(c.k), dev(c.v), dev(c.table), c.stride, c.n_pages, c.KV, c.hd)
+    start, past, out = dev(c.start), dev(np.array(c.past, np.int32)), torch.zeros(c.T, c.H * c.hd, device="cuda")
+    ws = torch.zeros(ab.ATTN_ROWS_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    call = lambda: ab.attention_packed(q, cache, start, past, 2, c.T, c.H, c.scale, out, ws, stream=s)
+    want, tol = ref.attention("packed", c.q, c.k, c.v, c.table, c.start, c.past, c.H, c.scale)
+    good = lambda: np.all(np.abs(host(out) - want) <= tol)
+elif what == "pages":
+    pool = torch.arange(4 * 64 * 8, dtype=torch.float32, device="cuda").view(4, 1, 64, 8)
+    want = host(pool).copy()
+    want[3] = want[1]
+    want[3, :, 5] = want[3, :, 9]
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    a1, a3, table, base, keep, ks = i(1), i(3), i(3), i(5), i(4), i(0, 1)
+    def call():
+        ab.kv_copy_pages([pool], 64 * 8, 4, a1, a3, 1, stream=s)
+        ab.kv_compact([pool], 4, 1, 8, table, 1, base, keep, ks, 1, 1, stream=s)
+    good = lambda: np.array_equal(host(pool), want)
+else:
+    rng = np.random.default_rng(3)
+    lg, u = rng.normal(0, 2, (3, 5000)).astype(np.float32), rng.random(3).astype(np.float32)
+    dl, du, tok = dev(lg), dev(u), torch.zeros(3, dtype=torch.int32, device="cuda")
+    call = lambda: ab.sample_rows(dl, 3, 5000, None, None, None, None, du, tok, stream=s)
+    good = lambda: list(host(tok)) == [ref.sample(lg[i], 1.0, 0, 1.0, 0.0, u[i]) for i in range(3)]
+torch.cuda.synchronize()
+with torch.cuda.stream(st):
+    g.capture_begin()
+    call()
+    g.capture_end()
+    g.replay()
+ab.device_sync()
+assert good(), what
+print("good")
+"""
+
+
+@pytest.mark.parametrize("what", ["attention48", "attention128", "attention160", "pages", "sample"])
+def test_the_first_call_of_a_process_can_be_captured(what):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    paths = [here, os.path.dirname(os.path.dirname(os.path.abspath(ab.__file__)))]
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(paths=paths), what], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "good" in r.stdout, r.stdout + r.stderr
+
+
 def test_offsets_past_32_bits():
     """Pages whose byte and element offsets need more than 32 bits."""
     import torch
@@ -291,6 +444,29 @@ def test_compact(arrays, KV, hd):
                     continue
                 p[table[s, b // 64], :, b % 64] = p[table[s, a // 64], :, a % 64]
         assert np.array_equal(host(t), p)
+
+
+def test_copy_more_pairs_than_a_grid_has_rows():
+    import torch
+    n = 70001
+    pool = torch.arange(2 * n * 4, dtype=torch.float32, device="cuda").view(2 * n, 4)
+    want = torch.cat([pool[:n], pool[:n].flip(0)])
+    dst = torch.arange(2 * n - 1, n - 1, -1, dtype=torch.int32, device="cuda")
+    ab.kv_copy_pages([pool], 4, 2 * n, torch.arange(n, dtype=torch.int32, device="cuda"), dst, n)
+    assert torch.equal(pool, want)
+
+
+def test_compaction_lists_that_make_no_sense_stay_in_bounds():
+    """Descending list ends, negative and far slots: the pool's other pages stay."""
+    rng = np.random.default_rng(9)
+    host_pool = rng.normal(0, 1, (6, 2, 64, 8)).astype(np.float32)
+    for start, keep, base in (([0, 3, 1], [5, -9, 2**31 - 1], [0, 10]), ([2, -2**31, 2**31 - 1], [1, 2, 3], [-5, 60]),
+                              ([-4, 2, 900], [2**31 - 1, -2**31, 0], [2**31 - 1, -2**31])):
+        d = dev(host_pool)
+        ab.kv_compact([d], 6, 2, 8, dev(np.array([[1], [2]], np.int32)), 1, dev(np.array(base, np.int32)),
+                      dev(np.array(keep, np.int32)), dev(np.array(start, np.int32)), 2, 3)
+        ab.device_sync()
+        assert np.array_equal(host(d)[[0, 3, 4, 5]], host_pool[[0, 3, 4, 5]])
 
 
 # ------------------------------------------------------------------- sampling
