@@ -25,9 +25,10 @@
 // step that crosses its target, gathers that step's few tokens in the first
 // CTA, sorts them and scans their masses. A step with more tokens than the
 // list holds (ties, far outliers) is narrowed by a radix descent over (logit
-// bits, id), 10 bits a pass. With top_k the first histogram only counts (one
-// shared-memory atomic a token in place of three, no exponential), and where
-// the tokens up to the k-th's step fit the list, one sort answers all.
+// bits, id), 10 bits a pass. With top_k the row is counted by fixed steps of
+// 1/16 of a logit while it is read, and where the tokens down to the k-th's
+// step fit the list (2048), one sort answers all; else the step of the k-th
+// token, of the steps of M - l, bounds the masses.
 #include "common.cuh"
 
 #include "device_check.hpp"
@@ -41,7 +42,8 @@ namespace
 
 constexpr int SR_THREADS = 1024, SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = 1024; // one per thread
-constexpr int SR_LIST = 512;
+constexpr int SR_LIST = 2048; // two a thread
+constexpr int SR_LOADS = 8; // a thread's loads in flight
 constexpr uint32_t SR_SLICE = 40000; // logits of a CTA in shared memory
 constexpr int SR_MASS_BITS = 45;
 
@@ -50,7 +52,8 @@ struct SrShared
     uint32_t cnt[SR_BINS], m0[SR_BINS], m1[SR_BINS], m2[SR_BINS]; // this CTA's histogram
     uint64_t pm[SR_BINS];                                         // cumulative mass of the row's steps
     uint32_t pc[SR_BINS];                                         // cumulative count
-    uint64_t lkey[SR_LIST], lmass[SR_LIST], skey[SR_LIST], smass[SR_LIST];
+    uint64_t lkey[SR_LIST]; // first CTA: the row's listed tokens, by order key
+    uint64_t lbuf[SR_LIST]; // this CTA's part of them; first CTA then: cumulative masses
     double tbl[64]; // 2^(j / 64)
     uint64_t wsum_m[SR_WARPS];
     uint32_t wsum_c[SR_WARPS];
@@ -58,7 +61,7 @@ struct SrShared
     uint32_t red_idx[SR_WARPS];
     float cta_max, cta_min;
     uint32_t cta_idx;
-    uint32_t n_list;
+    uint32_t n_list, n_mine, at_list;
     int pick;
     uint64_t above_m, tot_m;
     uint32_t above_c, n_in;
@@ -107,6 +110,12 @@ __device__ __forceinline__ uint64_t order_key(float l, uint32_t id)
     return ((uint64_t)o << 32) | (0xFFFFFFFFu - id);
 }
 
+__device__ __forceinline__ float order_logit(uint64_t key)
+{
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
+
 // exp(x) for -33 <= x <= 0 by table lookup (P. T. P. Tang, "Table-driven
 // implementation of the exponential function in IEEE floating-point
 // arithmetic", 1989): x = k ln2 / 64 + r, exp(x) = 2^(k / 64) exp(r), the
@@ -136,6 +145,13 @@ struct SrRow
 __device__ __forceinline__ int sr_bin(float l, const SrRow& r)
 {
     return min((int)((r.M - l) * r.invw), SR_BINS - 1); // monotone in l; NaN (0 * inf) counts as 0
+}
+
+// The step of 1/16 that a logit lies in, from +32 down to -32 (beyond: the end
+// ones): monotone like sr_bin, but needs no largest logit.
+__device__ __forceinline__ int sr_fixed_bin(float l)
+{
+    return min(max((int)((32.0f - l) * 16.0f), 0), SR_BINS - 1);
 }
 
 // mass in units of 2^-45; 0 for tokens below min_p
@@ -192,12 +208,13 @@ __device__ __forceinline__ void sr_clear(SrShared& s)
 
 __device__ __forceinline__ void sr_add(SrShared& s, int bin, uint64_t mass)
 {
-    if (mass)
-    {
-        atomicAdd(&s.m0[bin], (uint32_t)(mass & 0x7FFF));
-        atomicAdd(&s.m1[bin], (uint32_t)((mass >> 15) & 0x7FFF));
-        atomicAdd(&s.m2[bin], (uint32_t)(mass >> 30));
-    }
+    const uint32_t p0 = (uint32_t)mass & 0x7FFF, p1 = (uint32_t)(mass >> 15) & 0x7FFF, p2 = (uint32_t)(mass >> 30);
+    if (p0)
+        atomicAdd(&s.m0[bin], p0);
+    if (p1)
+        atomicAdd(&s.m1[bin], p1);
+    if (p2) // masses of 2^-15 of the largest and more
+        atomicAdd(&s.m2[bin], p2);
 }
 
 // The row's totals of bin threadIdx.x over the cluster's histograms.
@@ -232,57 +249,106 @@ __device__ __forceinline__ void sr_collect(SrShared& s, uint32_t& c, uint64_t& m
     }
 }
 
-// One token into the first CTA's list (what does not fit is counted only).
+// The counts alone of the row's bin threadIdx.x.
 template <int C>
-__device__ __forceinline__ void sr_append(SrShared& s, uint64_t key, uint64_t mass)
+__device__ __forceinline__ uint32_t sr_collect_counts(SrShared& s)
 {
     if constexpr (C == 1)
-    {
-        const uint32_t at = atomicAdd(&s.n_list, 1u);
-        if (at < (uint32_t)SR_LIST)
-        {
-            s.lkey[at] = key;
-            s.lmass[at] = mass;
-        }
-    }
-    else
-    {
-        const uint32_t at = peer_add32(peer_addr(&s.n_list, 0), 1u);
-        if (at < (uint32_t)SR_LIST)
-        {
-            peer_st64(peer_addr(&s.lkey[at], 0), key);
-            peer_st64(peer_addr(&s.lmass[at], 0), mass);
-        }
-    }
+        return s.cnt[threadIdx.x];
+    uint32_t v[C], c = 0;
+#pragma unroll
+    for (int r = 0; r < C; ++r)
+        v[r] = peer_ld32(peer_addr(&s.cnt[threadIdx.x], r));
+#pragma unroll
+    for (int r = 0; r < C; ++r)
+        c += v[r];
+    return c;
 }
 
-// The list's first n tokens in order into skey / smass: a token's place is how
-// many keys are larger (keys are distinct). Two threads count for a token.
+// One token into this CTA's part of the list (what does not fit is counted only).
+__device__ __forceinline__ void sr_append(SrShared& s, uint64_t key)
+{
+    const uint32_t at = atomicAdd(&s.n_mine, 1u);
+    if (at < (uint32_t)SR_LIST)
+        s.lbuf[at] = key;
+}
+
+// The CTAs' parts into the first CTA's list, in any order (it is sorted); n_list
+// counts what did not fit too.
+template <int C>
+__device__ __forceinline__ void sr_push(SrShared& s)
+{
+    __syncthreads();
+    const uint32_t n = s.n_mine;
+    if (threadIdx.x == 0)
+        s.at_list = C == 1 ? (s.n_list = n, 0u) : peer_add32(peer_addr(&s.n_list, 0), n);
+    __syncthreads();
+    const uint32_t at = s.at_list;
+    for (uint32_t i = threadIdx.x; i < min(n, (uint32_t)SR_LIST); i += SR_THREADS)
+        if (at + i < (uint32_t)SR_LIST)
+        {
+            if constexpr (C == 1)
+                s.lkey[at + i] = s.lbuf[i];
+            else
+                peer_st64(peer_addr(&s.lkey[at + i], 0), s.lbuf[i]);
+        }
+}
+
+// The list's first n tokens in order (keys are distinct). Up to 512 a token's
+// place is how many keys are larger, two threads counting for a token; more
+// take a bitonic network (2048: 66 steps, 15 of them over the whole CTA).
 __device__ __forceinline__ void sr_sort(SrShared& s, uint32_t n)
 {
-    static_assert(SR_THREADS == 2 * SR_LIST, "two threads a token");
-    const uint32_t i = threadIdx.x >> 1, part = threadIdx.x & 1;
-    uint32_t place = 0;
-    if (i < n)
+    const uint32_t t = threadIdx.x;
+    if (n <= SR_THREADS / 2)
     {
-        const uint64_t key = s.lkey[i];
+        const uint32_t i = t >> 1, part = t & 1;
+        uint32_t place = 0;
+        uint64_t key = 0;
+        if (i < n)
+        {
+            key = s.lkey[i];
 #pragma unroll 4
-        for (uint32_t j = part; j < n; j += 2)
-            place += s.lkey[j] > key;
+            for (uint32_t j = part; j < n; j += 2)
+                place += s.lkey[j] > key;
+        }
+        place += __shfl_xor_sync(0xffffffffu, place, 1);
+        __syncthreads();
+        if (i < n && part == 0)
+            s.lkey[place] = key;
+        __syncthreads();
+        return;
     }
-    place += __shfl_xor_sync(0xffffffffu, place, 1);
-    if (i < n && part == 0)
-    {
-        s.skey[place] = s.lkey[i];
-        s.smass[place] = s.lmass[i];
-    }
+    const uint32_t size = n <= SR_THREADS ? SR_THREADS : SR_LIST;
+    for (uint32_t i = n + t; i < size; i += SR_THREADS)
+        s.lkey[i] = 0; // behind every token
+    __syncthreads();
+    for (uint32_t block = 2; block <= size; block *= 2)
+        for (uint32_t step = block / 2; step > 0; step /= 2)
+        {
+            const uint32_t i = 2 * step * (t / step) + (t & (step - 1)), j = i + step;
+            if (j < size)
+            {
+                const uint64_t x = s.lkey[i], y = s.lkey[j];
+                if ((x < y) == ((i & block) == 0))
+                {
+                    s.lkey[i] = y;
+                    s.lkey[j] = x;
+                }
+            }
+            // up to 32 apart, the pairs of a warp are 64 tokens of its own, in this step and the next
+            if (step > 32 || (step == 1 && block >= 64))
+                __syncthreads();
+            else
+                __syncwarp();
+        }
     __syncthreads();
 }
 
 // C CTAs a row; RES: the slice's logits stay in shared memory, else every pass
 // reads them again (from L2 after the first).
 template <int C, bool RES>
-__global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const SampleRowsArgs a)
+__global__ void __launch_bounds__(SR_THREADS, RES ? 1 : 2) sample_rows_kernel(const SampleRowsArgs a)
 {
     extern __shared__ __align__(16) uint8_t sr_raw[];
     SrShared& s = *reinterpret_cast<SrShared*>(sr_raw);
@@ -293,17 +359,11 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
     const uint32_t v0 = rank * per, n_mine = v0 < a.vocab ? min(per, a.vocab - v0) : 0u;
     const float* src = a.logits + (size_t)row * a.ld + v0;
 
-    if constexpr (RES)
-    {
-        // a thread reads back only what it wrote
-#pragma unroll 8
-        for (uint32_t j = tid; j < n_mine; j += SR_THREADS)
-            slice[j] = __ldcs(src + j);
-    }
     // fn(logit, id) for each of this thread's tokens that is not NaN. Rolled:
     // unrolled over registers, the passes' code outgrew the instruction caches.
+    constexpr int UNROLL = RES ? 4 : 8;
     auto each = [&](auto&& fn) {
-#pragma unroll 2
+#pragma unroll UNROLL
         for (uint32_t j = tid; j < n_mine; j += SR_THREADS)
         {
             const float l = RES ? slice[j] : src[j];
@@ -312,21 +372,46 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         }
     };
 
+    const float T = a.temperature ? a.temperature[row] : 1.0f;
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const bool cut_k = k > 0 && (uint32_t)k < a.vocab && T > 0.0f;
     if (tid < 64)
         s.tbl[tid] = exp2((double)tid / 64.0);
     sr_clear(s);
-    // ---- the largest logit (its lowest id) and the smallest finite one
+    if (tid == 0)
+        s.n_list = s.n_mine = 0;
+    __syncthreads();
+    // ---- the row from memory: its largest logit (the lowest id of it) and the
+    // smallest finite one; with top_k the tokens of each 1/16 of a logit
     float mx = -INFINITY, mn = INFINITY;
     uint32_t mi = 0xFFFFFFFFu;
-    each([&](float l, uint32_t id) {
-        if (l > mx || (l == mx && id < mi))
+    for (uint32_t j0 = tid; j0 < n_mine; j0 += SR_THREADS * SR_LOADS)
+    {
+        float l[SR_LOADS];
+#pragma unroll
+        for (int u = 0; u < SR_LOADS; ++u)
+            l[u] = j0 + u * SR_THREADS < n_mine ? (RES ? __ldcs(src + j0 + u * SR_THREADS) : src[j0 + u * SR_THREADS])
+                                                : __uint_as_float(0x7FC00000u);
+#pragma unroll
+        for (int u = 0; u < SR_LOADS; ++u)
         {
-            mx = l;
-            mi = id;
+            const uint32_t j = j0 + u * SR_THREADS;
+            if (RES && j < n_mine)
+                slice[j] = l[u]; // read back by this thread only
+            if (l[u] == l[u])
+            {
+                if (l[u] > mx || mi == 0xFFFFFFFFu)
+                {
+                    mx = l[u];
+                    mi = v0 + j;
+                }
+                if (l[u] > -INFINITY)
+                    mn = fminf(mn, l[u]);
+                if (cut_k)
+                    atomicAdd(&s.cnt[sr_fixed_bin(l[u])], 1u);
+            }
         }
-        if (l > -INFINITY)
-            mn = fminf(mn, l);
-    });
+    }
     auto better = [](float& v, uint32_t& i, float ov, uint32_t oi) {
         if (ov > v || (ov == v && oi < i))
         {
@@ -375,7 +460,6 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
             mn = fminf(mn, __uint_as_float(peer_ld32(peer_addr(&s.cta_min, r))));
         }
     }
-    const float T = a.temperature ? a.temperature[row] : 1.0f;
     if (!(T > 0.0f) || !isfinite(mx))
     {
         // greedy (T <= 0), or no finite logit to normalise by
@@ -394,80 +478,88 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
     const float span = fminf(mx - mn, 40.0f * T);
     R.invw = span > 0.0f ? (float)SR_BINS / span : 0.0f;
 
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const bool cut_k = k > 0 && (uint32_t)k < a.vocab;
     const float tp = a.top_p ? a.top_p[row] : 1.0f;
     const float uu = a.u[row];
-    __syncthreads();
+    // the mass of the list's token i, i < n
+    auto mass_at = [&](uint32_t i, uint32_t n) -> uint64_t {
+        return i < n ? sr_mass(order_logit(s.lkey[i]), R, s.tbl) : 0ull;
+    };
     uint32_t c;
     uint64_t m;
     uint64_t key, W;
-    if (cut_k)
-    {
-        // ---- the step that holds the k-th token, by counts alone
-        each([&](float l, uint32_t) { atomicAdd(&s.cnt[sr_bin(l, R)], 1u); });
-        row_sync<C>();
-        sr_collect<C>(s, c, m);
+    // the step that holds the k-th token, by the counts of a histogram
+    auto pick_count = [&]() {
+        c = sr_collect_counts<C>(s);
         const uint32_t own = c;
-        sr_scan(c, m, s);
-        if (c >= (uint32_t)k && c - own < (uint32_t)k)
-        {
-            s.pick = tid;
-            s.n_in = c;
-        }
-        if (tid == 0)
-        {
-            s.n_list = 0;
-            if (c == 0)
-                s.n_in = 0;
-        }
+        uint64_t unused = 0;
+        sr_scan(c, unused, s);
         if (tid == SR_THREADS - 1 && c < (uint32_t)k) // fewer tokens than k (NaN logits): all of them
         {
             s.pick = SR_BINS - 1;
             s.n_in = c;
         }
-        row_sync<C>();
-        const int last = s.pick;
+        if (c >= (uint32_t)k && c - own < (uint32_t)k)
+        {
+            s.pick = tid;
+            s.n_in = c;
+        }
+        __syncthreads();
+    };
+    if (cut_k)
+    {
+        pick_count();
+        int last = s.pick;
         if (s.n_in <= (uint32_t)SR_LIST)
         {
             // everything that top_k can keep fits the list: one sort answers all
             each([&](float l, uint32_t id) {
-                if (sr_bin(l, R) <= last)
-                    sr_append<C>(s, order_key(l, id), sr_mass(l, R, s.tbl));
+                if (sr_fixed_bin(l) <= last)
+                    sr_append(s, order_key(l, id));
             });
+            sr_push<C>(s);
             row_sync<C>();
             if (rank == 0)
             {
-                const uint32_t n = min(s.n_list, (uint32_t)SR_LIST), kept = min(n, (uint32_t)k);
+                const uint32_t n = min(s.n_list, (uint32_t)SR_LIST), kept = min(n, (uint32_t)k), i = 2 * tid;
                 sr_sort(s, n);
+                const uint64_t m0 = mass_at(i, kept), m1 = mass_at(i + 1, kept);
                 uint32_t lc = 0;
-                uint64_t lm = tid < (int)kept ? s.smass[tid] : 0ull;
-                const uint64_t own_m = lm;
+                uint64_t lm = m0 + m1;
                 sr_scan(lc, lm, s);
-                if (tid < (int)kept)
-                    s.lmass[tid] = lm; // cumulative
+                s.lbuf[i] = lm - m1; // cumulative
+                s.lbuf[i + 1] = lm;
                 __syncthreads();
                 // first i with cum[i] >= target
                 auto cross = [&](double target) {
-                    const bool in = tid < (int)kept && (double)lm >= target;
-                    const bool before = tid < (int)kept && tid > 0 && (double)(lm - own_m) >= target;
-                    if (in && !before)
-                        s.pick = tid;
+#pragma unroll
+                    for (uint32_t e = i; e < i + 2; ++e)
+                        if (e < kept && (double)s.lbuf[e] >= target && !(e > 0 && (double)s.lbuf[e - 1] >= target))
+                            s.pick = e;
                     __syncthreads();
                     const int at = s.pick;
                     __syncthreads();
                     return at;
                 };
-                W = kept ? s.lmass[kept - 1] : 0ull;
+                W = kept ? s.lbuf[kept - 1] : 0ull;
                 if (tp < 1.0f)
-                    W = s.lmass[cross((double)tp * (double)W)];
+                    W = s.lbuf[cross((double)tp * (double)W)];
                 const int at = cross(uu > 0.0f ? fmin((double)uu, 1.0) * (double)W : 0.0);
                 if (tid == 0)
-                    a.tokens[row] = 0xFFFFFFFFu - (uint32_t)(s.skey[at] & 0xFFFFFFFFu);
+                    a.tokens[row] = 0xFFFFFFFFu - (uint32_t)(s.lkey[at] & 0xFFFFFFFFu);
             }
             return; // no CTA reads another's shared memory after the last barrier
         }
-        // more tokens than that: the masses of the steps up to the cut
+        // more tokens than that: the steps of M - l, first the one of the k-th
+        // token, then the masses up to it
+        row_sync<C>(); // the counts are read
+        sr_clear(s);
+        __syncthreads();
+        each([&](float l, uint32_t) { atomicAdd(&s.cnt[sr_bin(l, R)], 1u); });
+        row_sync<C>();
+        pick_count();
+        last = s.pick;
+        s.pc[tid] = c;
+        row_sync<C>();
         sr_clear(s);
         __syncthreads();
         each([&](float l, uint32_t) {
@@ -475,7 +567,6 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
             if (b <= last)
                 sr_add(s, b, sr_mass(l, R, s.tbl));
         });
-        s.pc[tid] = c;
     }
     else
         // ---- the masses of the 1024 steps of M - l
@@ -509,7 +600,7 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         pick_step(by_count ? s.pc[tid] : 0u, s.pm[tid], by_count && tid ? s.pc[tid - 1] : 0u, tid ? s.pm[tid - 1] : 0ull,
                   tid == 0);
         if (tid == 0)
-            s.n_list = 0;
+            s.n_list = s.n_mine = 0;
         __syncthreads();
         const int step = s.pick;
         uint32_t above_c = s.above_c;
@@ -526,9 +617,10 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
                 {
                     const uint64_t key = order_key(l, id);
                     if (mine(key))
-                        sr_append<C>(s, key, sr_mass(l, R, s.tbl));
+                        sr_append(s, key);
                 }
             });
+            sr_push<C>(s);
             row_sync<C>();
             const uint32_t n = C == 1 ? s.n_list : peer_ld32(peer_addr(&s.n_list, 0));
             if (n <= (uint32_t)SR_LIST || shift == 0)
@@ -557,7 +649,7 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
             if (own_c)
                 pick_step(above_c + dc, above_m + dm, above_c + dc - own_c, above_m + dm - own_m, dc == own_c);
             if (tid == 0)
-                s.n_list = 0;
+                s.n_list = s.n_mine = 0;
             __syncthreads();
             prefix |= (uint64_t)(SR_BINS - 1 - s.pick) << nshift;
             shift = nshift;
@@ -567,30 +659,34 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         }
         if (rank == 0)
         {
-            const uint32_t n = min(s.n_list, (uint32_t)SR_LIST);
+            const uint32_t n = min(s.n_list, (uint32_t)SR_LIST), i = 2 * tid;
             sr_sort(s, n);
-            uint32_t lc = tid < (int)n ? 1u : 0u;
-            uint64_t lm = tid < (int)n ? s.smass[tid] : 0ull;
-            const uint64_t own = lm;
-            sr_scan(lc, lm, s);
-            const bool in = by_count ? above_c + lc >= k : (double)(above_m + lm) >= target;
-            const bool before = tid == 0 ? false
-                                : by_count ? above_c + lc - 1 >= k
-                                           : (double)(above_m + lm - own) >= target;
-            if (tid < (int)n && ((in && !before) || (!in && tid == (int)n - 1)))
-            {
+            const uint64_t m0 = mass_at(i, n), m1 = mass_at(i + 1, n);
+            uint32_t unused = 0;
+            uint64_t lm = m0 + m1;
+            sr_scan(unused, lm, s);
 #pragma unroll
-                for (int r = 0; r < C; ++r)
+            for (uint32_t e = i; e < i + 2; ++e)
+            {
+                // mass up to and including token e, and before it
+                const uint64_t upto = above_m + (e == i ? lm - m1 : lm), under = upto - (e == i ? m0 : m1);
+                const bool in = by_count ? above_c + e + 1 >= k : (double)upto >= target;
+                const bool before = e > 0 && (by_count ? above_c + e >= k : (double)under >= target);
+                if (e < n && ((in && !before) || (!in && e == n - 1)))
                 {
-                    if constexpr (C == 1)
+#pragma unroll
+                    for (int r = 0; r < C; ++r)
                     {
-                        s.found_key = s.skey[tid];
-                        s.found_mass = above_m + lm;
-                    }
-                    else
-                    {
-                        peer_st64(peer_addr(&s.found_key, r), s.skey[tid]);
-                        peer_st64(peer_addr(&s.found_mass, r), above_m + lm);
+                        if constexpr (C == 1)
+                        {
+                            s.found_key = s.lkey[e];
+                            s.found_mass = upto;
+                        }
+                        else
+                        {
+                            peer_st64(peer_addr(&s.found_key, r), s.lkey[e]);
+                            peer_st64(peer_addr(&s.found_mass, r), upto);
+                        }
                     }
                 }
             }
@@ -655,12 +751,28 @@ int sample_rows(const SampleRowsArgs& a, cudaStream_t st)
         C *= 2;
     while (C < 8 && (size_t)a.rows * C * 2 <= (size_t)sm_count() && (a.vocab + C - 1) / C > 2048)
         C *= 2;
+    // More than four rounds of CTAs: two share an SM and hide each other's
+    // barriers, half as many a row, and read their slices again from L2 in every
+    // pass. By slices in shared memory and this way: 256 rows of 128256 172 us
+    // and 147, 512 337 and 234, 512 of 50257 150 and 116; 160 of 128256 (4.3
+    // rounds) 125 and 121, 96 73 and 101.
+    const bool many = (size_t)a.rows * C > 4 * (size_t)sm_count();
+    if (many && C > 1)
+        C /= 2;
+    if (many || (a.vocab + C - 1) / C > SR_SLICE)
+        switch (C)
+        {
+        case 1: return sr_launch<1, false>(a, st);
+        case 2: return sr_launch<2, false>(a, st);
+        case 4: return sr_launch<4, false>(a, st);
+        default: return sr_launch<8, false>(a, st);
+        }
     switch (C)
     {
     case 1: return sr_launch<1, true>(a, st);
     case 2: return sr_launch<2, true>(a, st);
     case 4: return sr_launch<4, true>(a, st);
-    default: return (a.vocab + 7) / 8 <= SR_SLICE ? sr_launch<8, true>(a, st) : sr_launch<8, false>(a, st);
+    default: return sr_launch<8, true>(a, st);
     }
 }
 

@@ -562,6 +562,30 @@ def test_sample_rows_agrees_with_the_one_row_sampler():
         assert _sample(lg, [0.8], None, [0.9], None, [u])[0] == host(tok)[0]
 
 
+@pytest.mark.parametrize("B,V", [(620, 3001), (300, 50257), (150, 128256), (76, 190001)])
+def test_sample_more_rows_than_the_gpu_holds(B, V):
+    """Several rounds of CTAs, for rows of one CTA and of more."""
+    rng = np.random.default_rng(B)
+    lg = rng.normal(0, 2, (B, V)).astype(np.float32)
+    lg[np.arange(B), rng.integers(0, V, B)] += rng.uniform(0, 9, B).astype(np.float32)
+    prm = _params(rng, B)
+    got, want = _sample(lg, *prm), _want(lg, *prm)
+    assert np.array_equal(got, want), np.argwhere(got != np.array(want))[:5]
+
+
+@pytest.mark.parametrize("V", [900, 5000, 40001])
+@pytest.mark.parametrize("k", [3, 300, 700, 1500, 2048, 2049, 4000])
+@pytest.mark.parametrize("spread,shift", [(2, 0), (0.001, 7.3), (80, 0), (3, -200)])
+def test_sample_top_k_of_any_size(V, k, spread, shift):
+    """Lists that are short, long and too long, of logits of any range."""
+    rng = np.random.default_rng(V + k)
+    lg = (rng.normal(0, spread, (4, V)) + shift).astype(np.float32)
+    T = [spread, 0.5 * spread, 2.0 * spread, 1.0]
+    p, m, u = [1.0, 0.9, 0.7, 1.0], [0.0, 0.0, 0.0, 0.01], rng.random(4).astype(np.float32) * np.float32(1 - 2.0 ** -24)
+    got, want = _sample(lg, T, [k] * 4, p, m, u), _want(lg, T, [k] * 4, p, m, u)
+    assert np.array_equal(got, want)
+
+
 def test_sample_rows_captured():
     import torch
     rng = np.random.default_rng(7)
