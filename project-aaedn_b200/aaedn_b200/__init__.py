@@ -7,6 +7,7 @@ entry point; build it with ``python project-aaedn_b200/build.py``.
 Device buffers can be any CUDA allocation (torch tensors are convenient:
 pass ``t.data_ptr()``); host buffers are numpy arrays.
 """
+import array
 import ctypes
 import os
 
@@ -408,8 +409,12 @@ def _arrays(d_arrays):
     if isinstance(d_arrays, ctypes.Array) or not len(d_arrays):
         return d_arrays or (_vp * 0)()
     if hasattr(d_arrays[0], "data_ptr"):
-        return (_vp * len(d_arrays))(*[a.data_ptr() for a in d_arrays])
-    return (_vp * len(d_arrays))(*[_p(a) for a in d_arrays])
+        flat = array.array("Q", [a.data_ptr() for a in d_arrays])
+    elif isinstance(d_arrays[0], int):
+        flat = array.array("Q", d_arrays)
+    else:
+        return (_vp * len(d_arrays))(*[_p(a) for a in d_arrays])
+    return (_vp * len(flat)).from_buffer(flat)  # quicker than from the numbers one by one
 
 
 def kv_copy_pages(d_arrays, page_floats, n_pages, d_src, d_dst, n, stream=None):

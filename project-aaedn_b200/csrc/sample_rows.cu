@@ -12,12 +12,11 @@
 // (top_k) or cumulative mass (top_p, the draw) reaches a target; min_p only
 // takes masses out of the sums.
 //
-// p is computed in fp64 (2^-52 relative; B200 runs fp64 at half the fp32
-// rate) and held as an integer number of units of 2^-45: sums of integers
-// are exact in any order, so the result does not depend on the order of the
-// atomics. The units' rounding moves a cumulative sum by at most 2^-46 a
-// token, below 2^-29 of the mass for a million tokens, and a uniform has 24
-// bits.
+// p is computed in fp64 (within 2^-47) and held as an integer number of units
+// of 2^-45: sums of integers are exact in any order, so the result does not
+// depend on the order of the atomics. The units' rounding moves a cumulative
+// sum by at most 2^-46 a token, below 2^-26 of the mass for a million tokens,
+// and a uniform has 24 bits.
 //
 // A row is a thread-block cluster of C CTAs, each with a slice of the
 // vocabulary in shared memory (one read of the logits). One pass makes a
@@ -54,7 +53,7 @@ struct SrShared
     uint32_t pc[SR_BINS];                                         // cumulative count
     uint64_t lkey[SR_LIST]; // first CTA: the row's listed tokens, by order key
     uint64_t lbuf[SR_LIST]; // this CTA's part of them; first CTA then: cumulative masses
-    double tbl[64]; // 2^(j / 64)
+    double tbl[128]; // 2^(j / 128)
     uint64_t wsum_m[SR_WARPS];
     uint32_t wsum_c[SR_WARPS];
     float red_max[SR_WARPS], red_min[SR_WARPS];
@@ -116,30 +115,11 @@ __device__ __forceinline__ float order_logit(uint64_t key)
     return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
 }
 
-// exp(x) for -33 <= x <= 0 by table lookup (P. T. P. Tang, "Table-driven
-// implementation of the exponential function in IEEE floating-point
-// arithmetic", 1989): x = k ln2 / 64 + r, exp(x) = 2^(k / 64) exp(r), the
-// polynomial of exp(r) to r^5 (|r| <= ln2 / 128: the next term is 4e-17).
-__device__ __forceinline__ double sr_exp(double x, const double* tbl)
-{
-    constexpr double LN2 = 0.69314718055994530942, MAGIC = 6755399441055744.0; // 1.5 * 2^52
-    const double t = fma(x, 64.0 / LN2, MAGIC);
-    const int k = __double2loint(t);
-    const double r = fma(t - MAGIC, -LN2 / 64.0, x);
-    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    const double y = tbl[k & 63] * p;
-    return __hiloint2double(__double2hiint(y) + (k >> 6) * (1 << 20), __double2loint(y));
-}
-
 struct SrRow
 {
     float M, invw;
-    double dM, inv_t, min_p;
-    float far; // M - l beyond which the mass rounds to zero units
+    double dM, per_t, min_p; // per_t: 128 / (T ln 2)
+    float far;               // M - l beyond which the mass rounds to zero units
 };
 
 __device__ __forceinline__ int sr_bin(float l, const SrRow& r)
@@ -154,16 +134,31 @@ __device__ __forceinline__ int sr_fixed_bin(float l)
     return min(max((int)((32.0f - l) * 16.0f), 0), SR_BINS - 1);
 }
 
-// mass in units of 2^-45; 0 for tokens below min_p
+// exp((l - M) / T) in units of 2^-45; 0 for tokens below min_p. Table lookup
+// (P. T. P. Tang, "Table-driven implementation of the exponential function in
+// IEEE floating-point arithmetic", 1989): (l - M) / T = (k + r) ln2 / 128 with
+// |r| <= 1/2, exp = 2^(k / 128) exp(r ln2 / 128), the polynomial to r^4 (its
+// next term is 1.2e-15, the rounding of per_t 33 * 2^-53: within 2^-47). l - M
+// is exact, so the largest logit has exactly 2^45 units. The fp64 rate bounds
+// the passes that need masses: ten fp64 instructions a token.
 __device__ __forceinline__ uint64_t sr_mass(float l, const SrRow& r, const double* tbl)
 {
     if (!(r.M - l <= r.far))
         return 0;
-    const double y = sr_exp(fmax(((double)l - r.dM) * r.inv_t, -33.0), tbl);
-    if (y < r.min_p)
+    constexpr double MAGIC = 6755399441055744.0, TWO52 = 4503599627370496.0; // 1.5 * 2^52, 2^52
+    constexpr double A = 0.69314718055994530942 / 128.0;
+    const double d = (double)l - r.dM, t = fma(d, r.per_t, MAGIC);
+    const int k = __double2loint(t);
+    const double f = fma(d, r.per_t, MAGIC - t);
+    double p = fma(f, A * A * A * A / 24.0, A * A * A / 6.0);
+    p = fma(p, f, A * A / 2.0);
+    p = fma(p, f, A);
+    p = fma(p, f, 1.0);
+    const double base = tbl[k & 127];
+    const double scaled = __hiloint2double(__double2hiint(base) + ((k >> 7) + SR_MASS_BITS) * (1 << 20), __double2loint(base));
+    if (r.min_p > 0.0 && scaled * p < r.min_p)
         return 0;
-    constexpr double TWO52 = 4503599627370496.0;
-    return (uint64_t)__double_as_longlong(fma(y, (double)(1ull << SR_MASS_BITS), TWO52)) & ((1ull << 52) - 1);
+    return (uint64_t)__double_as_longlong(fma(scaled, p, TWO52)) & ((1ull << 52) - 1);
 }
 
 // Inclusive scan over the CTA's threads of a count and a mass.
@@ -375,8 +370,8 @@ __global__ void __launch_bounds__(SR_THREADS, RES ? 1 : 2) sample_rows_kernel(co
     const float T = a.temperature ? a.temperature[row] : 1.0f;
     const int k = a.top_k ? a.top_k[row] : 0;
     const bool cut_k = k > 0 && (uint32_t)k < a.vocab && T > 0.0f;
-    if (tid < 64)
-        s.tbl[tid] = exp2((double)tid / 64.0);
+    if (tid < 128)
+        s.tbl[tid] = exp2((double)tid / 128.0);
     sr_clear(s);
     if (tid == 0)
         s.n_list = s.n_mine = 0;
@@ -471,10 +466,10 @@ __global__ void __launch_bounds__(SR_THREADS, RES ? 1 : 2) sample_rows_kernel(co
     SrRow R;
     R.M = mx;
     R.dM = (double)mx;
-    R.inv_t = 1.0 / (double)T;
+    R.per_t = 128.0 / 0.69314718055994530942 / (double)T;
     const float mp = a.min_p ? a.min_p[row] : 0.0f;
-    R.min_p = mp > 0.0f ? fmin((double)mp, 1.0) : 0.0;
-    R.far = 33.0f * T; // exp(-33) is below half a unit
+    R.min_p = mp > 0.0f ? fmin((double)mp, 1.0) * (double)(1ull << SR_MASS_BITS) : 0.0;
+    R.far = fminf(33.0f * T, 3.0e38f); // exp(-33) is below half a unit; an infinite distance is always far
     const float span = fminf(mx - mn, 40.0f * T);
     R.invw = span > 0.0f ? (float)SR_BINS / span : 0.0f;
 

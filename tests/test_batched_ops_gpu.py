@@ -586,6 +586,17 @@ def test_sample_top_k_of_any_size(V, k, spread, shift):
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("T", [float("inf"), 1e38, 1e-30, 1e-44])
+def test_sample_temperatures_at_the_ends(T):
+    rng = np.random.default_rng(10)
+    lg = rng.integers(-3, 4, (6, 3000)).astype(np.float32)
+    lg[:, ::7] = -np.inf
+    u = rng.random(6).astype(np.float32)
+    for k in (0, 100):
+        got, want = _sample(lg, [T] * 6, [k] * 6, None, None, u), _want(lg, [T] * 6, [k] * 6, None, None, u)
+        assert np.array_equal(got, want)
+
+
 def test_sample_rows_captured():
     import torch
     rng = np.random.default_rng(7)
