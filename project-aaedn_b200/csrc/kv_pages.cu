@@ -107,8 +107,8 @@ int kv_copy_pages_host(float* const* arrays, size_t n_arrays, size_t page_floats
 // rows loaded before the eight stores, and no other thread touches its
 // column. CTA (array, sequence). One layer's few rows are little work, so the
 // launch is what costs: 16 sequences, 24 slots each, 8 heads x 128 dims in 64
-// arrays 24 us, of which about 15 are the call's checks on the host; a launch
-// an array would be 64 of those.
+// arrays 19 us, most of them the call on the host; a launch an array would be
+// 64 of those.
 // ---------------------------------------------------------------------------
 constexpr int KP_THREADS = 256, KP_BATCH = 8;
 

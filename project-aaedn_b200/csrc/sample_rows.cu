@@ -340,6 +340,10 @@ __device__ __forceinline__ void sr_sort(SrShared& s, uint32_t n)
     __syncthreads();
 }
 
+// Bound by latencies (the cluster's barriers between a dozen passes) and, for
+// rows without top-k, by their masses in fp64: one row of 32000 12 us, 32 rows
+// of 128256 38 us, 256 rows 142 us (20 would be one read of the logits). A row
+// with top_k 50 takes 17 us of its cluster, one without top-k 25 to 35.
 // C CTAs a row; RES: the slice's logits stay in shared memory, else every pass
 // reads them again (from L2 after the first).
 template <int C, bool RES>
@@ -738,9 +742,10 @@ int sample_rows(const SampleRowsArgs& a, cudaStream_t st)
 {
     // The fewest CTAs a row whose shared memory holds it, then more while the
     // rows leave SMs idle and a CTA has over 2048 tokens. Measured at a
-    // vocabulary of 128256: 8 rows by 4 CTAs each 39 us, by 8 33; 32 rows by 4
-    // 41, by 8 63; 256 rows by 4 198, by 8 386 (each CTA's passes cost their
-    // barriers and histogram whatever its slice).
+    // vocabulary of 128256 (an earlier step, 32 rows now 38): 8 rows by 4 CTAs
+    // each 39 us, by 8 33; 32 rows by 4 41, by 8 63; 256 rows by 4 198, by 8
+    // 386 (each CTA's passes cost their barriers and histogram whatever its
+    // slice).
     int C = 1;
     while (C < 8 && (a.vocab + C - 1) / C > SR_SLICE)
         C *= 2;
