@@ -58,102 +58,183 @@ namespace aaedn_dev
 {
 
 // ---------------------------------------------------------------------------
-// One warp per (packed row, query head), for head_dim 129..256. Keys come 32
-// at a time: lane j scores key s0 + j against q (in shared memory), the softmax
-// is carried online (running max and sum), then the lanes take the head dims
-// and add the keys' weighted V rows. fp32 throughout; a key that the row may
-// not attend is never read, so what such a slot holds (NaN, an unused page) has
-// no effect. A row with no key gives zeros. Bound by its own loads: every row
-// reads its keys for itself, from L2 (1077 tokens, 16 heads of 256 dims: 2.9
-// ms).
+// head_dim 129..256: CTA = (up to 32 packed rows of one sequence, query head)
+// against tiles of 32 keys in shared memory, online softmax, fp32 throughout.
+// Warp w has rows w, w + 8, ...; lanes take the keys for the scores and the
+// dims for P V. Masked keys get no weight; a V row with a non-finite value is
+// zeros in shared memory and noted: a row that attends it becomes NaN, the
+// others never multiply it. A row with no key gives zeros. Bound by the tiles'
+// loads and barriers (8 us a tile where an SM has one CTA): 1077 rows, 16
+// heads of 256 dims 0.77 ms, eight trees of 16 over 900, 32 heads 0.44 ms; by a
+// warp a row that reads its keys for itself 2.9 and 1.3 ms (only single rows
+// over short caches, 64 over 200 keys, were faster that way: 0.29 against 0.56).
 // ---------------------------------------------------------------------------
-constexpr int RW_WARPS = 4;
+constexpr int RL_ROWS = 32, RL_KEYS = 32, RL_WARPS = 8, RL_RW = RL_ROWS / RL_WARPS, RL_LD = 256 + 4;
+constexpr size_t RL_SMEM = (size_t)(RL_ROWS + 2 * RL_KEYS) * RL_LD * 4;
 
 template <bool TREE>
-__global__ void __launch_bounds__(RW_WARPS * 32) attn_rows_warp_kernel(const AttnRowsArgs a)
+__global__ void __launch_bounds__(RL_WARPS * 32, 2) attn_rows_tile_kernel(const AttnRowsArgs a)
 {
-    __shared__ __align__(16) float qs[RW_WARPS][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x * RW_WARPS + warp, h = blockIdx.y;
-    if (row >= a.rows)
+    extern __shared__ __align__(16) float rl_smem[];
+    __shared__ unsigned bad[2]; // keys of a tile whose V is not finite, two tiles in turn
+    float* Qs = rl_smem;
+    float* Ks = Qs + RL_ROWS * RL_LD;
+    float* Vs = Ks + RL_KEYS * RL_LD;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    const int hd = a.head_dim, hd4 = hd >> 2, kvh = h / (a.n_heads / a.n_kv);
+    // the piece from packed row 32 x, or from the start of sequence x - blocks
+    // where that is inside a block of 32 rows: to the end of its block or sequence
+    const int blocks = (a.rows + RL_ROWS - 1) / RL_ROWS;
+    const bool starts = (int)blockIdx.x >= blocks;
+    const int r0 = starts ? a.row_start[blockIdx.x - blocks] : (int)blockIdx.x * RL_ROWS;
+    if (starts && (r0 < 0 || r0 >= a.rows || r0 % RL_ROWS == 0))
         return;
-    const int s = rows_seq_of(a, row);
+    const int s = starts ? (int)blockIdx.x - blocks : rows_seq_of(a, r0);
     if (s < 0)
         return;
-    const int hd = a.head_dim, kvh = h / (a.n_heads / a.n_kv);
-    const float* qr = a.q + (size_t)row * a.ldq + (size_t)h * hd;
-    for (int d = lane; d < hd; d += 32)
-        qs[warp][d] = qr[d];
-    __syncwarp();
-    const long long past = max(a.past[s], 0), cap = (long long)a.pt_stride * ROWS_PAGE;
-    const long long local = (long long)row - a.row_start[s];
+    const int first = a.row_start[s], r1 = min(min(a.rows, a.row_start[s + 1]), r0 / RL_ROWS * RL_ROWS + RL_ROWS);
+    if (r1 <= r0)
+        return;
+    const int np = r1 - r0;
+    const long long cap = (long long)a.pt_stride * ROWS_PAGE;
+    if (tid < 2)
+        bad[tid] = 0u;
+    unsigned turn = 0;
+    const long long past = max(a.past[s], 0);
     // keys 0..nk-1 are looked at
-    const long long nk = min(cap, TREE ? past + min((long long)a.mask_words * 64,
-                                                    (long long)min(a.row_start[s + 1], a.rows) - a.row_start[s])
-                                       : past + local + 1);
+    const long long nk = min(cap, TREE ? past + min((long long)a.mask_words * 64, (long long)min(a.row_start[s + 1], a.rows) - first)
+                                       : past + ((long long)r1 - first));
     const int* pt = rows_page_table(a, s);
-    const uint64_t* mask = TREE ? a.mask + (size_t)row * a.mask_words : nullptr;
-    auto kv_at = [&](const float* base, long long key) -> const float* {
-        const int page = pt[key / ROWS_PAGE];
-        if (page < 0 || page >= a.n_pages)
-            return nullptr; // not a page: as a masked key
-        return base + (((size_t)page * a.n_kv + kvh) * ROWS_PAGE + (size_t)(key % ROWS_PAGE)) * hd;
-    };
-    auto seen = [&](long long key) {
-        if (!TREE || key < past)
-            return true;
-        const int j = (int)(key - past);
-        return ((mask[j >> 6] >> (j & 63)) & 1) != 0;
-    };
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    float mrun = -INFINITY, lrun = 0.0f;
-    for (long long s0 = 0; s0 < nk; s0 += 32)
+    for (int i = tid; i < np * hd4; i += RL_WARPS * 32)
     {
-        const long long key = s0 + lane;
-        const float* kr = key < nk && seen(key) ? kv_at(a.k, key) : nullptr;
-        float sc = -INFINITY;
-        if (kr)
+        const int r = i / hd4, c = i - r * hd4;
+        *reinterpret_cast<float4*>(Qs + r * RL_LD + 4 * c) =
+            *reinterpret_cast<const float4*>(a.q + (size_t)(r0 + r) * a.ldq + (size_t)h * hd + 4 * c);
+    }
+    const int mine = (np - warp + RL_WARPS - 1) / RL_WARPS; // rows of this warp
+    float m[RL_RW], l[RL_RW];
+    float4 acc[RL_RW][2];
+#pragma unroll
+    for (int k = 0; k < RL_RW; ++k)
+    {
+        m[k] = -INFINITY;
+        l[k] = 0.0f;
+        acc[k][0] = acc[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (long long t0 = 0; t0 < nk; t0 += RL_KEYS)
+    {
+        const int page = pt[t0 / ROWS_PAGE];
+        if (page < 0 || page >= a.n_pages)
+            continue; // not a page: as masked keys
+        const size_t base = (((size_t)page * a.n_kv + kvh) * ROWS_PAGE + (size_t)(t0 % ROWS_PAGE)) * hd;
+        const int valid = (int)min((long long)RL_KEYS, nk - t0);
+        __syncthreads(); // the tile before is read
+#pragma unroll 4
+        for (int i = tid; i < RL_KEYS * hd4; i += RL_WARPS * 32)
         {
-            float dot = 0.0f;
-            for (int c = 0; c < (hd >> 2); ++c)
+            const int r = i / hd4, c = i - r * hd4;
+            float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
+            if (r < valid)
             {
-                const float4 kv = reinterpret_cast<const float4*>(kr)[c];
-                const float4 qv = reinterpret_cast<const float4*>(qs[warp])[c];
-                dot = fmaf(qv.x, kv.x, dot);
-                dot = fmaf(qv.y, kv.y, dot);
-                dot = fmaf(qv.z, kv.z, dot);
-                dot = fmaf(qv.w, kv.w, dot);
+                kv = *reinterpret_cast<const float4*>(a.k + base + (size_t)r * hd + 4 * c);
+                vv = *reinterpret_cast<const float4*>(a.v + base + (size_t)r * hd + 4 * c);
+                if (!(fabsf(vv.x) + fabsf(vv.y) + fabsf(vv.z) + fabsf(vv.w) < INFINITY) &&
+                    !(isfinite(vv.x) && isfinite(vv.y) && isfinite(vv.z) && isfinite(vv.w)))
+                {
+                    atomicOr(&bad[turn & 1u], 1u << r);
+                    vv = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
             }
-            sc = dot * a.scale;
+            *reinterpret_cast<float4*>(Ks + r * RL_LD + 4 * c) = kv;
+            *reinterpret_cast<float4*>(Vs + r * RL_LD + 4 * c) = vv;
         }
-        const float mnew = fmaxf(mrun, warp_max(sc));
-        const float ref = mnew == -INFINITY ? 0.0f : mnew; // nothing attended so far
-        const float w = kr ? expf(sc - ref) : 0.0f;
-        const float corr = expf(mrun - ref);
-        lrun = lrun * corr + warp_sum(w);
-        mrun = mnew;
+        if (tid == 0)
+            bad[(turn + 1u) & 1u] = 0u;
+        __syncthreads();
+        const unsigned nan_v = bad[turn & 1u];
+        ++turn;
+        const long long key = t0 + lane;
+        float w[RL_RW];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            acc[i] *= corr;
-        const unsigned live = __ballot_sync(0xffffffffu, kr != nullptr);
-        for (int j = 0; j < 32; ++j)
+        for (int k = 0; k < RL_RW; ++k)
+            w[k] = 0.0f;
+        for (int c = 0; c < hd4; ++c)
         {
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            if (!((live >> j) & 1))
-                continue;
-            const float* vr = kv_at(a.v, s0 + j);
+            const float4 kf = *reinterpret_cast<const float4*>(Ks + lane * RL_LD + 4 * c);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (lane + 32 * i < hd)
-                    acc[i] = fmaf(wj, vr[lane + 32 * i], acc[i]);
+            for (int k = 0; k < RL_RW; ++k)
+                if (k < mine)
+                {
+                    const float4 qf = *reinterpret_cast<const float4*>(Qs + (k * RL_WARPS + warp) * RL_LD + 4 * c);
+                    w[k] = fmaf(qf.x, kf.x, w[k]);
+                    w[k] = fmaf(qf.y, kf.y, w[k]);
+                    w[k] = fmaf(qf.z, kf.z, w[k]);
+                    w[k] = fmaf(qf.w, kf.w, w[k]);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < RL_RW; ++k)
+        {
+            if (k >= mine)
+                continue;
+            const int row = r0 + k * RL_WARPS + warp;
+            bool see = lane < valid;
+            if (!TREE)
+                see = see && key <= past + ((long long)row - first);
+            else if (see && key >= past)
+            {
+                const int j = (int)(key - past);
+                see = ((a.mask[(size_t)row * a.mask_words + (j >> 6)] >> (j & 63)) & 1) != 0;
+            }
+            const float sc = see ? w[k] * a.scale : -INFINITY;
+            const float mnew = fmaxf(m[k], warp_max(sc)), ref = mnew == -INFINITY ? 0.0f : mnew;
+            const float corr = expf(m[k] - ref);
+            m[k] = mnew;
+            w[k] = see ? expf(sc - ref) : 0.0f;
+            l[k] = l[k] * corr + warp_sum(w[k]);
+            if ((__ballot_sync(0xffffffffu, see) & nan_v) != 0u)
+                l[k] = __uint_as_float(0x7FC00000u);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                acc[k][e].x *= corr;
+                acc[k][e].y *= corr;
+                acc[k][e].z *= corr;
+                acc[k][e].w *= corr;
+            }
+        }
+        for (int j = 0; j < valid; ++j)
+        {
+            const float4 v0 = *reinterpret_cast<const float4*>(Vs + j * RL_LD + 4 * lane);
+            const float4 v1 = *reinterpret_cast<const float4*>(Vs + j * RL_LD + 128 + 4 * lane);
+#pragma unroll
+            for (int k = 0; k < RL_RW; ++k)
+                if (k < mine)
+                {
+                    const float wj = __shfl_sync(0xffffffffu, w[k], j);
+                    acc[k][0].x = fmaf(wj, v0.x, acc[k][0].x);
+                    acc[k][0].y = fmaf(wj, v0.y, acc[k][0].y);
+                    acc[k][0].z = fmaf(wj, v0.z, acc[k][0].z);
+                    acc[k][0].w = fmaf(wj, v0.w, acc[k][0].w);
+                    acc[k][1].x = fmaf(wj, v1.x, acc[k][1].x);
+                    acc[k][1].y = fmaf(wj, v1.y, acc[k][1].y);
+                    acc[k][1].z = fmaf(wj, v1.z, acc[k][1].z);
+                    acc[k][1].w = fmaf(wj, v1.w, acc[k][1].w);
+                }
         }
     }
-    const float inv = lrun == 0.0f ? 0.0f : 1.0f / lrun;
-    float* o = a.out + (size_t)row * a.ldo + (size_t)h * hd;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < hd)
-            o[lane + 32 * i] = acc[i] * inv;
+    for (int k = 0; k < RL_RW; ++k)
+        if (k < mine)
+        {
+            const float inv = l[k] == 0.0f ? 0.0f : 1.0f / l[k];
+            float* o = a.out + (size_t)(r0 + k * RL_WARPS + warp) * a.ldo + (size_t)h * hd;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (e * 32 + lane < hd4)
+                    *reinterpret_cast<float4*>(o + e * 128 + 4 * lane) =
+                        make_float4(acc[k][e].x * inv, acc[k][e].y * inv, acc[k][e].z * inv, acc[k][e].w * inv);
+        }
 }
 
 template <typename Kern>
@@ -172,6 +253,10 @@ int attn_rows_init()
     static PerDeviceOnce once;
     return once.run([]() -> int {
         int rc;
+        AAEDN_CUDA_TRY(cudaFuncSetAttribute(attn_rows_tile_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)RL_SMEM));
+        AAEDN_CUDA_TRY(cudaFuncSetAttribute(attn_rows_tile_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)RL_SMEM));
         if ((rc = rows_tc_attrs(attn_rows_tc_kernel<false>, RT_SMEM)) ||
             (rc = rows_tc_attrs(attn_rows_tc_kernel<true>, RT_SMEM)) ||
             (rc = rows_tc_attrs(attn_rows_pair_kernel<false>, RP_SMEM)))
@@ -290,26 +375,25 @@ static int rows_tc_launch(const AttnRowsArgs& a, cudaStream_t st)
 // us, by the pairs 131; a tree of 16 over 4001 tokens 26, by the pairs 34).
 // 65..128 the pairs (a prompt of 4096 tokens, 64 heads over 8: 924 us when they
 // came, by single SMs 1053; eight sequences of 4120 tokens 259 and 274).
-// Above, a tile's operands do not fit one SM's tensor memory beside its sums:
-// one warp a row (on prompts 70 to 90 times slower where both can run: 13.6
-// against 0.15 ms; only calls of a few rows over short caches lose nothing by
-// it: 5 rows without a cache 16 us, by the pairs 20).
+// Above, a tile's operands and sums do not fit one SM's tensor memory: fp32 on
+// the FMA units. (Where both run, one warp a row, the simplest kernel, was 70 to
+// 90 times slower than the tensor cores on prompts: 13.6 against 0.15 ms.)
 int attn_rows(const AttnRowsArgs& a, cudaStream_t st)
 {
+    if (int rc = attn_rows_init())
+        return rc;
     if (a.head_dim <= 128)
     {
-        if (int rc = attn_rows_init())
-            return rc;
         if (a.head_dim <= 64)
             return a.mask ? rows_tc_launch<true>(a, st) : rows_tc_launch<false>(a, st);
         return a.mask ? rows_pair_launch<true>(a, st) : rows_pair_launch<false>(a, st);
     }
-    const dim3 grid((unsigned)((a.rows + RW_WARPS - 1) / RW_WARPS), (unsigned)a.n_heads);
+    const dim3 tiles((unsigned)((a.rows + RL_ROWS - 1) / RL_ROWS + a.n_seqs), (unsigned)a.n_heads);
     if (a.mask)
-        attn_rows_warp_kernel<true><<<grid, RW_WARPS * 32, 0, st>>>(a);
+        attn_rows_tile_kernel<true><<<tiles, RL_WARPS * 32, RL_SMEM, st>>>(a);
     else
-        attn_rows_warp_kernel<false><<<grid, RW_WARPS * 32, 0, st>>>(a);
-    AAEDN_LAUNCH_CHECK("attn_rows_warp_kernel");
+        attn_rows_tile_kernel<false><<<tiles, RL_WARPS * 32, RL_SMEM, st>>>(a);
+    AAEDN_LAUNCH_CHECK("attn_rows_tile_kernel");
     return AAEDN_OK;
 }
 

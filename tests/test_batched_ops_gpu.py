@@ -364,6 +364,27 @@ def test_the_first_call_of_a_process_can_be_captured(what):
     assert r.returncode == 0 and "good" in r.stdout, r.stdout + r.stderr
 
 
+@pytest.mark.parametrize("hd", [132, 256])
+def test_wide_heads(hd):
+    """The cases above on the kernel for head_dim above 128."""
+    test_infinities_and_nan_reach_the_rows_that_attend_them_only(hd)
+    test_pages_outside_the_pool_and_slots_behind_the_table_are_left_out(hd)
+    test_values_of_any_size(hd)
+    test_thousands_of_sequences(hd)
+
+
+def test_wide_heads_with_index_arrays_that_make_no_sense():
+    import torch
+    c = ref.Case(4, 2, 136, [20, 20], [64, 10], seed=32, poison=False)
+    for start, past in (([0, 30, 20], [64, 10]), ([5, 10, 4000], [-7, -100]), ([-3, 8, 40], [2**31 - 1, 5]),
+                        ([40, 20, 0], [0, 0]), ([2**31 - 1, -2**31, 7], [1, 1]), ([9, -2**31, 2**31 - 1], [3, 3])):
+        out = torch.full((40, c.H * c.hd), 7.0, device="cuda")
+        cache = ab.KvCache(dev(c.k), dev(c.v), dev(c.table), c.stride, c.n_pages, c.KV, c.hd)
+        ab.attention_packed(dev(c.q), cache, dev(np.array(start, np.int32)), dev(np.array(past, np.int32)), 2, 40, c.H,
+                            c.scale, out, _workspace())
+        ab.device_sync()
+
+
 def test_offsets_past_32_bits():
     """Pages whose byte and element offsets need more than 32 bits."""
     import torch
