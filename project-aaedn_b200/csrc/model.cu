@@ -2930,37 +2930,11 @@ extern "C" int aaedn_model_step_tree(aaedn_model* m, const uint32_t* h_seqs, con
     return device_status(m);
 }
 
-extern "C" int aaedn_seq_accept(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts,
-                                const uint32_t* h_nodes, size_t n)
+// Moves the kept nodes of n sequences (pf_rows in all at most) to the front of
+// their drafts and drops the rest.
+static int accept_group(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts, const uint32_t* h_nodes,
+                        size_t n)
 {
-    BATCHED_OK(m);
-    const char* fn = "aaedn_seq_accept";
-    if (!h_seqs || !h_counts || n == 0 || n > m->max_seqs)
-        return set_error(AAEDN_EINVAL, "%s: 1..%u sequences", fn, m->max_seqs);
-    std::vector<uint8_t> seen(m->max_seqs, 0);
-    size_t total = 0;
-    for (size_t i = 0; i < n; ++i)
-    {
-        if (int rc = seq_ok(m, h_seqs[i]))
-            return rc;
-        if (seen[h_seqs[i]]++)
-            return set_error(AAEDN_EINVAL, "sequence %u twice in one batch", h_seqs[i]);
-        const auto& draft = m->seqs[h_seqs[i]].draft;
-        if (draft.empty())
-            return set_error(AAEDN_ESTATE, "%s: sequence %u has no drafted tree", fn, h_seqs[i]);
-        if (h_counts[i] && !h_nodes)
-            return set_error(AAEDN_EINVAL, "%s: null nodes", fn);
-        int32_t prev = -1;
-        for (uint32_t j = 0; j < h_counts[i]; ++j)
-        {
-            const uint32_t node = h_nodes[total + j];
-            if (node >= draft.size() || draft[node] != prev)
-                return set_error(AAEDN_EINVAL, "%s: node %u of sequence %u does not follow node %d", fn, node, h_seqs[i],
-                                 prev);
-            prev = (int32_t)node;
-        }
-        total += h_counts[i];
-    }
     AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream)); // the staging may still feed an earlier copy
     const RowsPlan &h = m->h_plan, &d = m->d_plan;
     size_t t = 0;
@@ -3001,6 +2975,53 @@ extern "C" int aaedn_seq_accept(aaedn_model* m, const uint32_t* h_seqs, const ui
         m->seqs[h_seqs[i]].len += h_counts[i];
         if (int rc = trim(m, h_seqs[i]))
             return rc;
+    }
+    return AAEDN_OK;
+}
+
+extern "C" int aaedn_seq_accept(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts,
+                                const uint32_t* h_nodes, size_t n)
+{
+    BATCHED_OK(m);
+    const char* fn = "aaedn_seq_accept";
+    if (!h_seqs || !h_counts || n == 0 || n > m->max_seqs)
+        return set_error(AAEDN_EINVAL, "%s: 1..%u sequences", fn, m->max_seqs);
+    std::vector<uint8_t> seen(m->max_seqs, 0);
+    size_t total = 0;
+    for (size_t i = 0; i < n; ++i)
+    {
+        if (int rc = seq_ok(m, h_seqs[i]))
+            return rc;
+        if (seen[h_seqs[i]]++)
+            return set_error(AAEDN_EINVAL, "sequence %u twice in one batch", h_seqs[i]);
+        const auto& draft = m->seqs[h_seqs[i]].draft;
+        if (draft.empty())
+            return set_error(AAEDN_ESTATE, "%s: sequence %u has no drafted tree", fn, h_seqs[i]);
+        if (h_counts[i] && !h_nodes)
+            return set_error(AAEDN_EINVAL, "%s: null nodes", fn);
+        int32_t prev = -1;
+        for (uint32_t j = 0; j < h_counts[i]; ++j)
+        {
+            const uint32_t node = h_nodes[total + j];
+            if (node >= draft.size() || draft[node] != prev)
+                return set_error(AAEDN_EINVAL, "%s: node %u of sequence %u does not follow node %d", fn, node, h_seqs[i],
+                                 prev);
+            prev = (int32_t)node;
+        }
+        total += h_counts[i];
+    }
+    // The plan's lists hold pf_rows entries: one step_tree stays below that (a
+    // sequence's draft too), the drafts of several calls need not, so the
+    // sequences are taken in groups that do.
+    size_t node0 = 0; // the group's first node in h_nodes
+    for (size_t i0 = 0, i1; i0 < n; i0 = i1)
+    {
+        size_t nodes = 0;
+        for (i1 = i0; i1 < n && nodes + h_counts[i1] <= (size_t)m->pf_rows; ++i1)
+            nodes += h_counts[i1];
+        if (int rc = accept_group(m, h_seqs + i0, h_counts + i0, h_nodes + node0, i1 - i0))
+            return rc;
+        node0 += nodes;
     }
     return AAEDN_OK;
 }
