@@ -13,10 +13,12 @@
 // takes masses out of the sums.
 //
 // p is computed in fp64 (within 2^-47) and held as an integer number of units
-// of 2^-45: sums of integers are exact in any order, so the result does not
-// depend on the order of the atomics. The units' rounding moves a cumulative
-// sum by at most 2^-46 a token, below 2^-26 of the mass for a million tokens,
-// and a uniform has 24 bits.
+// of 2^-44: sums of integers are exact in any order, so the result does not
+// depend on the order of the atomics. A million tokens as likely as the largest
+// are below 2^64 units. The units' rounding moves a cumulative sum by at most
+// 2^-45 a token, below 2^-25 of the mass for a million tokens, and a uniform
+// has 24 bits. A step's sum in a CTA is in three 32-bit parts of 15, 15 and 14
+// bits a token, so a CTA's slice is at most 131071 tokens.
 //
 // A row is a thread-block cluster of C CTAs, each with a slice of the
 // vocabulary in shared memory (one read of the logits). One pass makes a
@@ -44,7 +46,13 @@ constexpr int SR_BINS = 1024; // one per thread
 constexpr int SR_LIST = 2048; // two a thread
 constexpr int SR_LOADS = 8; // a thread's loads in flight
 constexpr uint32_t SR_SLICE = 40000; // logits of a CTA in shared memory
-constexpr int SR_MASS_BITS = 45;
+constexpr int SR_MASS_BITS = 44;
+constexpr uint32_t SR_MAX_SLICE = 131071; // tokens of a CTA
+static_assert(((uint64_t)SR_MAX_VOCAB << SR_MASS_BITS) >> SR_MASS_BITS == SR_MAX_VOCAB, "a row's mass");
+static_assert((uint64_t)SR_MAX_SLICE * 0x7FFF <= 0xFFFFFFFFull &&
+                  ((uint64_t)SR_MAX_SLICE << (SR_MASS_BITS - 30)) <= 0xFFFFFFFFull,
+              "a step's mass parts");
+static_assert((SR_MAX_VOCAB + 7) / 8 <= SR_MAX_SLICE, "8 CTAs a row at most");
 
 struct SrShared
 {
@@ -134,12 +142,12 @@ __device__ __forceinline__ int sr_fixed_bin(float l)
     return min(max((int)((32.0f - l) * 16.0f), 0), SR_BINS - 1);
 }
 
-// exp((l - M) / T) in units of 2^-45; 0 for tokens below min_p. Table lookup
+// exp((l - M) / T) in units of 2^-44; 0 for tokens below min_p. Table lookup
 // (P. T. P. Tang, "Table-driven implementation of the exponential function in
 // IEEE floating-point arithmetic", 1989): (l - M) / T = (k + r) ln2 / 128 with
 // |r| <= 1/2, exp = 2^(k / 128) exp(r ln2 / 128), the polynomial to r^4 (its
 // next term is 1.2e-15, the rounding of per_t 33 * 2^-53: within 2^-47). l - M
-// is exact, so the largest logit has exactly 2^45 units. The fp64 rate bounds
+// is exact, so the largest logit has exactly 2^44 units. The fp64 rate bounds
 // the passes that need masses: ten fp64 instructions a token.
 __device__ __forceinline__ uint64_t sr_mass(float l, const SrRow& r, const double* tbl)
 {
@@ -757,7 +765,7 @@ int sample_rows(const SampleRowsArgs& a, cudaStream_t st)
     // and 147, 512 337 and 234, 512 of 50257 150 and 116; 160 of 128256 (4.3
     // rounds) 125 and 121, 96 73 and 101.
     const bool many = (size_t)a.rows * C > 4 * (size_t)sm_count();
-    if (many && C > 1)
+    if (many && C > 1 && (a.vocab + C / 2 - 1) / (C / 2) <= SR_MAX_SLICE)
         C /= 2;
     if (many || (a.vocab + C - 1) / C > SR_SLICE)
         switch (C)

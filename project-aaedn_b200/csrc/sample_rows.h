@@ -22,7 +22,7 @@ struct SampleRowsArgs
     uint32_t* tokens;         // [rows]
 };
 
-constexpr uint32_t SR_MAX_VOCAB = 1000000; // the top mass part of a CTA's slice stays below 2^32
+constexpr uint32_t SR_MAX_VOCAB = 1000000; // a row's mass stays below 2^64 units (sample_rows.cu)
 
 int sample_rows(const SampleRowsArgs& a, cudaStream_t st);
 
