@@ -77,6 +77,7 @@ struct RpShared
     float q_down[4][128]; // what undoes an item's rows' scaling of Q
     uint64_t seen[4][128]; // which of a unit's keys a row attends
     float2 stats[4][128]; // (sum, offset) of an item's rows
+    float lo[4][128]; // and the second part of a far offset
 };
 
 // ---- the pair -------------------------------------------------------------------
@@ -403,7 +404,8 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
             float qf = 0.0f;
             const int limit = TREE ? c.q.past : min(c.q.past, INT_MAX - c.q.n) + r; // past + r: far behind cap when clamped
             const uint64_t* mask = TREE ? a.mask + (size_t)(c.q.begin + (live ? r : 0)) * a.mask_words : nullptr;
-            // weights are held as exp2(s + off) = 2^14 exp(score - max)
+            // weights are held as exp2(s + off) = 2^14 exp(score - max); a far offset
+            // has a second part in sm.lo
             float off = INFINITY, l = 0.0f;
             bool bad = false;
             for (int u = c.u0; u < c.u1; ++u, ++g)
@@ -427,8 +429,8 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                     qf = qs * sm.q_down[item & 3u][i];
                 // keys 0..31 and 32..63 were scaled by the two CTAs
                 const uint4 in = *reinterpret_cast<const uint4*>(sm.kinfo[g % RP_INFO]); // (down, bad) twice
-                const float fa = fmaxf(qf * __uint_as_float(in.x), 1.17549435e-38f);
-                const float fb = fmaxf(qf * __uint_as_float(in.z), 1.17549435e-38f);
+                float fa = rt_score_scale(qf * __uint_as_float(in.x));
+                float fb = rt_score_scale(qf * __uint_as_float(in.z));
                 const uint64_t seen = live ? rt_seen<TREE>(u, sm.valid[g % RP_INFO], limit, mask, a.mask_words) : 0ull;
                 sm.seen[g & 3u][i] = seen;
                 if ((in.y | in.w) != 0u && (seen & ((uint64_t)in.y | (uint64_t)in.w << 32)) != 0ull)
@@ -448,8 +450,20 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                     top = fmaxf(top, rt_max16(s) * (j0 < 32 ? fa : fb));
                 }
                 const float noff = fminf(off, 14.0f - top);
-                const float use = noff < INFINITY ? noff : 0.0f;
-                const float corr = rt_exp2(use - off); // 0 before the first key
+                float use = noff < INFINITY ? noff : 0.0f, corr = use - off;
+                if (__any_sync(0xffffffffu, fabsf(use) > RT_FAR || rt_far(off)))
+                {
+                    const bool far = fabsf(use) > RT_FAR;
+                    const float2 r = rt_far_unit(ts, seen, far ? fa : 1.0f, far ? fb : 1.0f, far ? use : 0.0f, off,
+                                                 &sm.lo[item & 3u][i]);
+                    corr += r.x;
+                    if (far)
+                    {
+                        use = r.y;
+                        fa = fb = 1.0f;
+                    }
+                }
+                corr = rt_exp2(corr); // 0 before the first key
                 off = noff;
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -565,7 +579,11 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                 float* slot = rt_slot<HDP>(a, blockIdx.x, item == 0 ? 0 : 1);
                 to = slot + (size_t)i * HDP + d_first;
                 if (d_first == 0)
+                {
                     reinterpret_cast<float2*>(slot + 128 * HDP)[i] = make_float2(l, stat.y);
+                    if (rt_far(stat.y))
+                        slot[128 * HDP + 256 + i] = sm.lo[item & 3u][i];
+                }
             }
             // a row a thread: whole 32-byte sectors where the addresses allow it
             if (((uint32_t)reinterpret_cast<uintptr_t>(to) & 31u) == 0u && (n & 7) == 0)

@@ -174,11 +174,12 @@ struct RtStart
 };
 
 constexpr size_t RT_HEADER_BYTES = 64 * 1024;
-// partial sums: [CTA][2][128 rows][HDP], then [CTA][2][128 rows] (sum, offset)
+// partial sums: [CTA][2] of [128 rows][HDP], [128 rows] (sum, offset) and [128 rows]
+// of the second part of a far offset
 template <int HDP>
 __host__ __device__ inline size_t rt_slot_bytes()
 {
-    return (size_t)128 * HDP * 4 + 128 * 8;
+    return (size_t)128 * HDP * 4 + 128 * 12;
 }
 template <int HDP>
 __device__ __forceinline__ float* rt_slot(const AttnRowsArgs& a, int cta, int which)
@@ -350,6 +351,15 @@ __device__ __forceinline__ void rt_ld<16>(uint32_t taddr, float* v)
         v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void rt_ld8(uint32_t taddr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 __device__ __forceinline__ void rt_st8(uint32_t taddr, const uint32_t (&r)[8])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
@@ -510,6 +520,7 @@ struct RtShared
     float q_down[4][128]; // what undoes an item's rows' scaling of Q
     uint64_t seen[4][128]; // which of a unit's keys a row attends
     float2 stats[4][128]; // (sum, offset) of an item's rows
+    float lo[4][128]; // and the second part of a far offset
 };
 
 // i / G for i < 128 and G <= 64, by the reciprocal in 2^-16 (kernel-wide
@@ -528,6 +539,10 @@ __device__ __forceinline__ long long rt_row_at(const RtSeq& q, int h, int t, int
         return -1;
     return (long long)((size_t)(q.begin + r) * ld + (size_t)(h * G + i - tok * G) * hd);
 }
+
+// What a score of the scaled factors is times scale log2(e): a normal number (a
+// key of zeros has the score 0, not NaN, next to the largest ones).
+__device__ __forceinline__ float rt_score_scale(float f) { return fminf(fmaxf(f, 1.17549435e-38f), 3.40282347e+38f); }
 
 // scores of keys that a row does not attend
 __device__ __forceinline__ void rt_mask16(float (&s)[16], uint32_t seen)
@@ -568,6 +583,44 @@ __device__ __forceinline__ float2 rt_weights(const float (&s)[16], float f, floa
     rt_st8(t, hi);
     rt_st8(t + 8, lo);
     return rt_add2(part[0], part[1]);
+}
+
+// Offsets above this are far: 14 - top and s f + off are then no longer both near
+// the exact value (spacings of 1/8 and more in exp2's argument; at 2^25 the weights
+// would leave the range of fp16), so a far offset is the sum of two floats. That
+// costs 2 % where no row is far, the vote on it: one prompt of 2048 tokens, 32
+// heads, 148 us from 145, a tree batch 134.4 from 133.9.
+constexpr float RT_FAR = 1048576.0f;
+__device__ __forceinline__ bool rt_far(float off) { return fabsf(off) > RT_FAR && off < INFINITY; }
+
+// Before the weights of a unit with far rows: their scores in tensor memory become
+// fma(s, f, use), one rounding of the exact value, whose largest gives the second
+// part of the offset, in *lo from here on (off: the first part before this unit).
+// Other rows come with f = 1 and use = 0. Returns the second parts' difference
+// and the new one. A call: hardly ever run, its code would crowd the loops.
+__device__ __noinline__ float2 rt_far_unit(uint32_t ts, uint64_t seen, float fa, float fb, float use, float off, float* lo)
+{
+    float top = -INFINITY;
+#pragma unroll 1
+    for (uint32_t j0 = 0; j0 < 64; j0 += 8)
+    {
+        uint32_t w[8];
+        rt_ld8(ts + j0, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+        {
+            const float x = fmaf(__uint_as_float(w[j]), j0 < 32 ? fa : fb, use);
+            w[j] = __float_as_uint(x);
+            top = (uint32_t)(seen >> j0) >> j & 1u ? fmaxf(top, x) : top;
+        }
+        rt_st8(ts + j0, w);
+    }
+    rt_wait_st();
+    const float old = rt_far(off) ? *lo : 0.0f;
+    float now = 0.0f;
+    if (use != 0.0f)
+        *lo = now = fminf(use == off ? old : INFINITY, 14.0f - top);
+    return make_float2(now - old, now);
 }
 
 // Which of the 64 keys of a unit a row attends. limit: causal: the row's last
@@ -855,7 +908,8 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             float qf = 0.0f;
             const int limit = TREE ? c.q.past : min(c.q.past, INT_MAX - c.q.n) + r; // past + r: far behind cap when clamped
             const uint64_t* mask = TREE ? a.mask + (size_t)(c.q.begin + (live ? r : 0)) * a.mask_words : nullptr;
-            // weights are held as exp2(s + off) = 2^14 exp(score - max)
+            // weights are held as exp2(s + off) = 2^14 exp(score - max); a far offset
+            // has a second part in sm.lo
             float off = INFINITY, l = 0.0f;
             bool bad = false;
             for (int u = c.u0; u < c.u1; ++u, ++g)
@@ -871,7 +925,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 if (u == c.u0)
                     qf = qs * sm.q_down[item & 3u][i];
                 const RtUnitInfo& in = sm.info[g % RT_INFO];
-                const float f = fmaxf(qf * in.k_down, 1.17549435e-38f);
+                float f = rt_score_scale(qf * in.k_down);
                 const uint64_t seen = live ? rt_seen<TREE>(u, in.valid, limit, mask, a.mask_words) : 0ull;
                 sm.seen[g & 3u][i] = seen;
                 if ((in.kbad[0] | in.kbad[1]) != 0u &&
@@ -892,8 +946,20 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     top = fmaxf(top, rt_max16(s) * f);
                 }
                 const float noff = fminf(off, 14.0f - top);
-                const float use = noff < INFINITY ? noff : 0.0f;
-                const float corr = rt_exp2(use - off); // 0 before the first key
+                float use = noff < INFINITY ? noff : 0.0f, corr = use - off;
+                if (__any_sync(0xffffffffu, fabsf(use) > RT_FAR || rt_far(off)))
+                {
+                    const bool far = fabsf(use) > RT_FAR;
+                    const float2 r = rt_far_unit(ts, seen, far ? f : 1.0f, far ? f : 1.0f, far ? use : 0.0f, off,
+                                                 &sm.lo[item & 3u][i]);
+                    corr += r.x;
+                    if (far)
+                    {
+                        use = r.y;
+                        f = 1.0f;
+                    }
+                }
+                corr = rt_exp2(corr); // 0 before the first key
                 off = noff;
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -998,7 +1064,11 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 float* slot = rt_slot<HDP>(a, blockIdx.x, item == 0 ? 0 : 1);
                 to = slot + (size_t)i * HDP + d_first;
                 if (d_first == 0)
+                {
                     reinterpret_cast<float2*>(slot + 128 * HDP)[i] = make_float2(l, stat.y);
+                    if (rt_far(stat.y))
+                        slot[128 * HDP + 256 + i] = sm.lo[item & 3u][i];
+                }
             }
             // a row a thread: whole 32-byte sectors where the addresses allow it
             if (((uint32_t)reinterpret_cast<uintptr_t>(to) & 31u) == 0u && (n & 7) == 0)
@@ -1239,6 +1309,42 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
 // ---------------------------------------------------------------------------
 constexpr int RJ_WARPS = 8;
 
+// A row with a far least offset, to `o` (one warp): the shares from `first` on that
+// have units of the tile [t0, t1), one after the other, with the second parts of
+// their offsets.
+template <int HDP, int NC>
+__device__ __noinline__ void rt_join_far(const AttnRowsArgs& a, int grid, int first, int part, int i, unsigned long long t0,
+                                         unsigned long long t1, float off, float* o)
+{
+    const int lane = threadIdx.x & 31;
+    const RtStart* starts = reinterpret_cast<const RtStart*>(a.workspace);
+    float lo = INFINITY, l = 0.0f, acc[HDP / 32] = {};
+    for (int turn = 0; turn < 2; ++turn) // the least second part that goes with off; the sums
+        for (int c = first; c < grid && starts[c].begin < t1; ++c)
+        {
+            if (starts[c].begin >= starts[c + 1].begin)
+                continue;
+            const float* slot = rt_slot<HDP>(a, c * NC + part, starts[c].begin >= t0 ? 0 : 1);
+            const float2 s = __ldcg(reinterpret_cast<const float2*>(slot + 128 * HDP) + i);
+            const float second = rt_far(s.y) ? __ldcg(slot + 128 * HDP + 256 + i) : 0.0f;
+            if (turn == 0)
+            {
+                lo = s.y == off ? fminf(lo, second) : lo;
+                continue;
+            }
+            const float w = s.y < INFINITY ? rt_exp2((off - s.y) + (lo - second)) : 0.0f;
+            l += s.x * w;
+#pragma unroll
+            for (int d = 0; d < HDP / 32; ++d)
+                acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), w, acc[d]);
+        }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+        if (d * 32 + lane < a.head_dim)
+            o[d * 32 + lane] = acc[d] * inv;
+}
+
 // NC CTAs work on a share together (128 rows each).
 template <int HDP, bool TREE, int NC>
 __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const AttnRowsArgs a, int grid)
@@ -1278,6 +1384,12 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
     float off = -warp_max(-s.y);
     for (int c = first + 32; more; c += 32)
         off = fminf(off, -warp_max(-stat_of(c, more).y));
+    float* o = a.out + (size_t)(q.begin + r) * a.ldo + (size_t)(st.h * G + (i - ti * G)) * a.head_dim;
+    if (rt_far(off))
+    {
+        rt_join_far<HDP, NC>(a, grid, first, part, i, t0, t1, off, o);
+        return;
+    }
     float l = 0.0f, acc[HDP / 32];
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
@@ -1315,7 +1427,6 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float* o = a.out + (size_t)(q.begin + r) * a.ldo + (size_t)(st.h * G + (i - ti * G)) * a.head_dim;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
         if (d * 32 + lane < a.head_dim)

@@ -41,3 +41,70 @@ def test_sample_flat_rows_of_the_largest_vocabularies(B, V):
     few = slice(0, min(B, 8))  # no cut at all
     got, want = _sample(lg, T, None, None, None, u), _want(lg[few], T[few], None, None, None, u[few])
     assert np.array_equal(got[few], want)
+
+
+def _far_case(H, KV, hd, rows, past, sign, bits, seed):
+    """Scores of about sign * 2^(2 bits - 1) whose differences are whole
+    multiples of their spacing in fp32. q and k are whole numbers with few
+    bits, so every product and every sum of them
+    is exact in fp32 in any order and in parts of 11 bits."""
+    c = ref.Case(H, KV, hd, rows, past, seed=seed)
+    rng = np.random.default_rng(seed)
+    used = np.isfinite(c.k[:, 0, :, 0])
+    big, step = 2.0 ** bits, 2.0 ** (2 * bits - 23)
+    q = np.zeros((c.T, H, hd), np.float32)
+    q[:, :, 0] = big / 2 + rng.integers(0, 2 ** (bits - 3), (c.T, H))
+    q[:, :, 1:4] = step
+    k = np.zeros_like(c.k)
+    k[..., 0] = sign * big
+    k[..., 1:4] = rng.integers(-1, 2, k.shape[:-1] + (3,))
+    c.q = q.reshape(c.T, H * hd)
+    c.k = np.where(used[:, None, :, None], k, c.k)
+    c.scale = 1.0
+    return c
+
+
+def _check_far(c, kind, got, masks=None):
+    """The scores are exact (above), so only the weights' arithmetic counts: a
+    weight's argument x (in powers of two below the row's largest) passes a
+    scale of 2^-23, up to four roundings of 2^-24 and an exponential of 2^-22.
+    Weights from 2^-32 on count: 32 * 0.7 * (2^-23 + 4 * 2^-24) + 2^-22 <
+    2^-17 of a weight, 2^-19 more as in ref.attention (its own bits, the sums),
+    twice that of the mean of |v|, and 2^-37 of the largest |v|."""
+    want, _ = ref.attention(kind, c.q, c.k, c.v, c.table, c.start, c.past, c.H, c.scale, masks)
+    vabs, _ = ref.attention(kind, c.q, c.k, np.abs(c.v), c.table, c.start, c.past, c.H, c.scale, masks)
+    top = np.abs(c.v[np.isfinite(c.v)]).max()
+    tol = (2.0 ** -17 + 2.0 ** -19) * 2 * vabs + top * 2.0 ** -37
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (bad.mean(), np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
+
+
+@pytest.mark.parametrize("hd", [48, 128, 160])
+@pytest.mark.parametrize("sign,bits", [(1, 12), (1, 13), (-1, 13), (1, 15), (-1, 15)])
+def test_scores_of_any_size(hd, sign, bits):
+    """Scores of 2^23, 2^25 and 2^29, of either sign: over one unit of keys and over
+    several, in tiles that the shares of the work cut and in whole ones."""
+    for rows, past in (([40], [0]), ([70, 3, 100], [100, 200, 1]), ([1 + i % 3 for i in range(700)], [40] * 700)):
+        c = _far_case(4, 2, hd, rows, past, sign, bits, seed=hd + bits)
+        _check_far(c, "packed", _call(c, "packed"))
+
+
+@pytest.mark.parametrize("hd", [64, 96, 132])
+def test_scores_of_any_size_under_masks(hd):
+    """Rows of huge and of ordinary scores in one tile, rows without a key, keys
+    of the largest score masked."""
+    c = _far_case(4, 2, hd, [30, 9], [0, 130], 1, 13, seed=hd)
+    q = c.q.reshape(c.T, 4, hd)
+    q[::3] = np.random.default_rng(1).normal(0, 1e-4, q[::3].shape)  # ordinary scores
+    q[::3, :, 0] = 2.0 ** -13
+    masks = ref.masks_of(ref.random_parents(np.random.default_rng(2), 39), 1)
+    masks[30:] = ref.masks_of(ref.random_parents(np.random.default_rng(3), 9), 1)
+    masks[4:7] = 0
+    masks[11] = 0b100010
+    got = _call(c, "tree", masks)
+    want, tol = ref.attention("tree", c.q, c.k, c.v, c.table, c.start, c.past, c.H, c.scale, masks)
+    ordinary = np.arange(c.T) % 3 == 0
+    assert np.all(np.abs(got - want)[ordinary] <= tol[ordinary])
+    assert np.all(got[4:7] == 0)
+    c.q[ordinary] = 0.0  # compared above: uniform weights in what follows
+    _check_far(c, "tree", _call(c, "tree", masks), masks)
