@@ -564,14 +564,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
             if (!any)
                 continue;
             const float l = bad ? __uint_as_float(0x7FC00000u) : stat.x;
+            // the row's mean, of a cut tile too: the sums of values near the largest fp32
+            // pass it. In this order: 1 / l of the sums is at most 2^15, unit / l of small
+            // values would be denormal.
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
             float* to;
-            float by = unit;
             int n = W; // dims to store
             if (c.whole)
             {
                 const long long at = rt_row_at(c.q, c.h, 2 * c.t + (int)rank, i, G, R, a.ldo, hd);
                 to = a.out + at + d_first;
-                by = l == 0.0f ? 0.0f : unit / l;
                 n = at < 0 ? 0 : hd - d_first;
             }
             else
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
 #pragma unroll
                 for (int d = 0; d < W; d += 8)
                     if (d < n)
-                        rt_store8(to + d, acc + d, by);
+                        rt_store8(to + d, acc + d, by, unit);
             }
             else
             {
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                 for (int d = 0; d < W; d += 4)
                     if (d < n)
                         *reinterpret_cast<float4*>(to + d) =
-                            make_float4(acc[d] * by, acc[d + 1] * by, acc[d + 2] * by, acc[d + 3] * by);
+                            make_float4(acc[d] * by * unit, acc[d + 1] * by * unit, acc[d + 2] * by * unit, acc[d + 3] * by * unit);
             }
         }
         failed = !ok;

@@ -25,7 +25,7 @@
 // Work split: the units of all (sequence, K/V head, tile) in a row are cut
 // into equal shares, one persistent CTA (or pair) each, so long prompts, many
 // short ones and a small tree over a long cache all fill the GPU. A tile that
-// a cut goes through is written as partial sums (at most two a CTA) that a
+// a cut goes through is written as partial means (at most two a CTA) that a
 // second kernel joins, in a fixed order: no atomics, the same bits every time.
 //
 // Roles (28 warps, 1 CTA an SM): warp 0 copies pages (bulk copies into a ring
@@ -174,7 +174,7 @@ struct RtStart
 };
 
 constexpr size_t RT_HEADER_BYTES = 64 * 1024;
-// partial sums: [CTA][2] of [128 rows][HDP], [128 rows] (sum, offset) and [128 rows]
+// partial means: [CTA][2] of [128 rows][HDP], [128 rows] (sum, offset) and [128 rows]
 // of the second part of a far offset
 template <int HDP>
 __host__ __device__ inline size_t rt_slot_bytes()
@@ -437,11 +437,12 @@ __device__ __forceinline__ void rt_split2(float x, float y, uint32_t& hi, uint32
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
 }
 
-// p[0..7] = v[0..7] * by, p 32-byte aligned
-__device__ __forceinline__ void rt_store8(float* p, const float* v, float by)
+// p[0..7] = v[0..7] * by * unit, p 32-byte aligned
+__device__ __forceinline__ void rt_store8(float* p, const float* v, float by, float unit)
 {
-    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0] * by), "f"(v[1] * by),
-                 "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by), "f"(v[7] * by)
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0] * by * unit),
+                 "f"(v[1] * by * unit), "f"(v[2] * by * unit), "f"(v[3] * by * unit), "f"(v[4] * by * unit),
+                 "f"(v[5] * by * unit), "f"(v[6] * by * unit), "f"(v[7] * by * unit)
                  : "memory");
 }
 
@@ -1049,14 +1050,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
             if (!ok)
                 break;
             const float l = bad ? __uint_as_float(0x7FC00000u) : stat.x;
+            // the row's mean, of a cut tile too: the sums of values near the largest fp32
+            // pass it. In this order: 1 / l of the sums is at most 2^15, unit / l of small
+            // values would be denormal.
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
             float* to;
-            float by = unit;
             int n = W; // dims to store
             if (c.whole)
             {
                 const long long at = rt_row_at(c.q, c.h, c.t, i, G, R, a.ldo, hd);
                 to = a.out + at + d_first;
-                by = l == 0.0f ? 0.0f : unit / l;
                 n = at < 0 ? 0 : hd - d_first;
             }
             else
@@ -1076,7 +1079,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
 #pragma unroll
                 for (int d = 0; d < W; d += 8)
                     if (d < n)
-                        rt_store8(to + d, acc + d, by);
+                        rt_store8(to + d, acc + d, by, unit);
             }
             else
             {
@@ -1084,7 +1087,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                 for (int d = 0; d < W; d += 4)
                     if (d < n)
                         *reinterpret_cast<float4*>(to + d) =
-                            make_float4(acc[d] * by, acc[d + 1] * by, acc[d + 2] * by, acc[d + 3] * by);
+                            make_float4(acc[d] * by * unit, acc[d + 1] * by * unit, acc[d + 2] * by * unit, acc[d + 3] * by * unit);
             }
         }
         failed = !ok;
@@ -1302,7 +1305,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
 }
 
 // ---------------------------------------------------------------------------
-// Joins the partial sums of the tiles that a share's end went through: CTA
+// Joins the partial means of the tiles that a share's end went through: CTA
 // (boundary c, 8 rows), one row a warp. The tile's shares are taken in order.
 // At most two slots a CTA, 38 MB in all, from L2 behind two dependent loads:
 // 13 us after eight sequences of 4120 tokens, by itself and from cold caches.
@@ -1318,8 +1321,9 @@ __device__ __noinline__ void rt_join_far(const AttnRowsArgs& a, int grid, int fi
 {
     const int lane = threadIdx.x & 31;
     const RtStart* starts = reinterpret_cast<const RtStart*>(a.workspace);
-    float lo = INFINITY, l = 0.0f, acc[HDP / 32] = {};
-    for (int turn = 0; turn < 2; ++turn) // the least second part that goes with off; the sums
+    float lo = INFINITY, l = 0.0f, inv = 0.0f, acc[HDP / 32];
+    for (int turn = 0; turn < 3; ++turn) // the least second part that goes with off; the sum; the mean
+    {
         for (int c = first; c < grid && starts[c].begin < t1; ++c)
         {
             if (starts[c].begin >= starts[c + 1].begin)
@@ -1332,17 +1336,22 @@ __device__ __noinline__ void rt_join_far(const AttnRowsArgs& a, int grid, int fi
                 lo = s.y == off ? fminf(lo, second) : lo;
                 continue;
             }
-            const float w = s.y < INFINITY ? rt_exp2((off - s.y) + (lo - second)) : 0.0f;
-            l += s.x * w;
+            const float w = s.y < INFINITY ? s.x * rt_exp2((off - s.y) + (lo - second)) : 0.0f;
+            l += turn == 1 ? w : 0.0f;
+            if (turn == 2)
 #pragma unroll
-            for (int d = 0; d < HDP / 32; ++d)
-                acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), w, acc[d]);
+                for (int d = 0; d < HDP / 32; ++d)
+                    acc[d] = fmaf(__ldcg(slot + (size_t)i * HDP + d * 32 + lane), w * inv, acc[d]);
         }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < HDP / 32; ++d)
+            acc[d] = turn < 2 ? 0.0f * inv : acc[d];
+    }
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
         if (d * 32 + lane < a.head_dim)
-            o[d * 32 + lane] = acc[d] * inv;
+            o[d * 32 + lane] = acc[d];
 }
 
 // NC CTAs work on a share together (128 rows each).
@@ -1379,9 +1388,10 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         more = __all_sync(0xffffffffu, b < t1);
         return v;
     };
-    bool more;
-    float2 s = stat_of(first, more);
-    float off = -warp_max(-s.y);
+    bool more, more0;
+    const float2 s0 = stat_of(first, more0); // mostly all of them
+    float off = -warp_max(-s0.y);
+    more = more0;
     for (int c = first + 32; more; c += 32)
         off = fminf(off, -warp_max(-stat_of(c, more).y));
     float* o = a.out + (size_t)(q.begin + r) * a.ldo + (size_t)(st.h * G + (i - ti * G)) * a.head_dim;
@@ -1390,18 +1400,30 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
         rt_join_far<HDP, NC>(a, grid, first, part, i, t0, t1, off, o);
         return;
     }
-    float l = 0.0f, acc[HDP / 32];
-#pragma unroll
-    for (int d = 0; d < HDP / 32; ++d)
-        acc[d] = 0.0f;
-    more = true;
-    for (int c = first; more; c += 32)
+    // what a share's mean counts: its sum at the least offset, over all of them
+    float2 s = s0;
+    auto weight = [&]() -> float { return s.y < INFINITY ? s.x * rt_exp2(off - s.y) : s.x; };
+    float l = warp_sum(weight());
+    more = more0;
+    for (int c = first + 32; more; c += 32)
     {
         s = stat_of(c, more);
-        const float w = s.y < INFINITY ? rt_exp2(off - s.y) : 0.0f;
-        l += warp_sum(s.x * w);
+        l += warp_sum(weight());
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float acc[HDP / 32];
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+        acc[d] = 0.0f * inv; // NaN where no key counts but a query is NaN
+    s = s0;
+    more = more0;
+    for (int c = first;; c += 32)
+    {
+        if (c > first)
+            s = stat_of(c, more);
+        const float w = weight() * inv;
         unsigned has = __ballot_sync(0xffffffffu, s.y < INFINITY);
-        // in order, four shares' sums loaded before the first is used
+        // in order, four shares' means loaded before the first is used
         while (has)
         {
             float v[4][HDP / 32], wj[4];
@@ -1425,12 +1447,13 @@ __global__ void __launch_bounds__(RJ_WARPS * 32) attn_rows_join_kernel(const Att
                 for (int d = 0; d < HDP / 32; ++d)
                     acc[d] = fmaf(v[k][d], wj[k], acc[d]);
         }
+        if (!more)
+            break;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
         if (d * 32 + lane < a.head_dim)
-            o[d * 32 + lane] = acc[d] * inv;
+            o[d * 32 + lane] = acc[d];
 }
 
 } // namespace aaedn_dev

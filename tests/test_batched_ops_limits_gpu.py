@@ -108,3 +108,26 @@ def test_scores_of_any_size_under_masks(hd):
     assert np.all(got[4:7] == 0)
     c.q[ordinary] = 0.0  # compared above: uniform weights in what follows
     _check_far(c, "tree", _call(c, "tree", masks), masks)
+
+
+def _check_scaled(c, kind, got, masks=None):
+    want, tol = ref.attention(kind, c.q, c.k, c.v, c.table, c.start, c.past, c.H, c.scale, masks)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (bad.mean(), np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [1e-33, 1e34, 5e37])
+def test_values_near_the_ends_of_their_range(hd, size):
+    """The mean of values that fp32 holds, where their sum and the sum of their
+    scaled parts need not be: in tiles that the shares cut and in whole ones.
+    (Values of up to 5 * 5e37 < 3.4e38; from 2^-112 up a value's parts lose
+    nothing to its range, so the bounds are the usual ones.)"""
+    for rows, past in (([200, 9], [57, 1000]), ([1 + i % 3 for i in range(700)], [90] * 700)):
+        c = ref.Case(4, 2, hd, rows, past, seed=hd)
+        c.v = (c.v.astype(np.float64) * size).astype(np.float32)
+        _check_scaled(c, "packed", _call(c, "packed"))
+    masks = ref.masks_of(ref.random_parents(np.random.default_rng(4), 20), 1)
+    c = ref.Case(8, 2, hd, [20], [3000], seed=hd + 1)
+    c.v = (c.v.astype(np.float64) * size).astype(np.float32)
+    _check_scaled(c, "tree", _call(c, "tree", masks), masks)
