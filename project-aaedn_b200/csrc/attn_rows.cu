@@ -112,13 +112,16 @@ __global__ void __launch_bounds__(RL_WARPS * 32, 2) attn_rows_tile_kernel(const 
             *reinterpret_cast<const float4*>(a.q + (size_t)(r0 + r) * a.ldq + (size_t)h * hd + 4 * c);
     }
     const int mine = (np - warp + RL_WARPS - 1) / RL_WARPS; // rows of this warp
-    float m[RL_RW], l[RL_RW];
+    // the weights are held in units that keep their sum at 1 or less, and so every
+    // sum of the values within their range
+    float m[RL_RW], l[RL_RW], unit[RL_RW];
     float4 acc[RL_RW][2];
 #pragma unroll
     for (int k = 0; k < RL_RW; ++k)
     {
         m[k] = -INFINITY;
         l[k] = 0.0f;
+        unit[k] = 1.0f;
         acc[k][0] = acc[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (long long t0 = 0; t0 < nk; t0 += RL_KEYS)
@@ -188,10 +191,19 @@ __global__ void __launch_bounds__(RL_WARPS * 32, 2) attn_rows_tile_kernel(const 
             }
             const float sc = see ? w[k] * a.scale : -INFINITY;
             const float mnew = fmaxf(m[k], warp_max(sc)), ref = mnew == -INFINITY ? 0.0f : mnew;
-            const float corr = expf(m[k] - ref);
+            float corr = expf(m[k] - ref);
             m[k] = mnew;
-            w[k] = see ? expf(sc - ref) : 0.0f;
+            w[k] = see ? expf(sc - ref) * unit[k] : 0.0f;
             l[k] = l[k] * corr + warp_sum(w[k]);
+            if (l[k] > 1.0f)
+            {
+                // by a power of two, which is exact, to at most 1
+                const float down = __uint_as_float((253u - (__float_as_uint(l[k]) >> 23)) << 23);
+                unit[k] *= down;
+                corr *= down;
+                w[k] *= down;
+                l[k] *= down;
+            }
             if ((__ballot_sync(0xffffffffu, see) & nan_v) != 0u)
                 l[k] = __uint_as_float(0x7FC00000u);
 #pragma unroll

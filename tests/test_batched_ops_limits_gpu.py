@@ -131,3 +131,9 @@ def test_values_near_the_ends_of_their_range(hd, size):
     c = ref.Case(8, 2, hd, [20], [3000], seed=hd + 1)
     c.v = (c.v.astype(np.float64) * size).astype(np.float32)
     _check_scaled(c, "tree", _call(c, "tree", masks), masks)
+
+
+@pytest.mark.parametrize("hd", [132, 256])
+@pytest.mark.parametrize("size", [1e-33, 1e34, 5e37])
+def test_wide_heads_values_near_the_ends_of_their_range(hd, size):
+    test_values_near_the_ends_of_their_range(hd, size)
