@@ -2359,13 +2359,13 @@ static void release_pages(aaedn_model* m, std::vector<int>& pages)
     pages.clear();
 }
 
-// Gives back the pages behind sequence seq's last token (what a draft that
-// was not accepted, or a call that failed, left reserved).
-static int trim(aaedn_model* m, uint32_t seq)
+// Drops the draft of sequence seq and gives back the pages (of that draft, or of
+// a call that failed: nobody else's) that positions [0, len + n) do not need.
+static int drop_draft(aaedn_model* m, uint32_t seq, uint32_t n)
 {
     auto& sq = m->seqs[seq];
     sq.draft.clear();
-    const size_t need = ((size_t)sq.len + m->page_size - 1) / m->page_size;
+    const size_t need = ((size_t)sq.len + n + m->page_size - 1) / m->page_size;
     if (sq.pages.size() <= need)
         return AAEDN_OK;
     std::vector<int> rest(sq.pages.begin() + (ptrdiff_t)need, sq.pages.end());
@@ -2373,6 +2373,8 @@ static int trim(aaedn_model* m, uint32_t seq)
     release_pages(m, rest);
     return upload_pt(m, seq);
 }
+
+static int trim(aaedn_model* m, uint32_t seq) { return drop_draft(m, seq, 0); }
 
 // Enqueues the page copies that reserve() collected: one launch for every
 // layer's K and V.
@@ -2389,15 +2391,12 @@ static int flush_copies(aaedn_model* m)
 
 // Pages for positions [len, len + n) of sequence seq: new pages from the
 // pool, and a copy of the page holding position len when another sequence
-// shares it (its rows below len stay valid in both). A draft that was not
-// accepted is dropped. The copies are enqueued by flush_copies.
+// shares it (its rows below len stay valid in both). The copies are enqueued
+// by flush_copies.
 static int reserve(aaedn_model* m, uint32_t seq, uint32_t n)
 {
     auto& sq = m->seqs[seq];
     const uint32_t P = (uint32_t)m->page_size;
-    sq.draft.clear();
-    if ((size_t)sq.len + n > m->cfg.max_seq)
-        return set_error(AAEDN_ESTATE, "sequence %u full: %u + %u tokens > max_seq %u", seq, sq.len, n, m->cfg.max_seq);
     bool changed = false;
     if (n && sq.len % P != 0)
     {
@@ -2444,10 +2443,17 @@ static int reserve(aaedn_model* m, uint32_t seq, uint32_t n)
     return rc;
 }
 
-// reserve() for several sequences; on a failure the pages of the earlier
-// ones are given back.
+// reserve() for several sequences, whose drafts are dropped first; on a failure
+// the pages of the earlier ones are given back.
 static int reserve_all(aaedn_model* m, const uint32_t* seqs, const uint32_t* counts, size_t n)
 {
+    for (size_t i = 0; i < n; ++i)
+        if ((size_t)m->seqs[seqs[i]].len + (counts ? counts[i] : 1u) > m->cfg.max_seq)
+            return set_error(AAEDN_ESTATE, "sequence %u full: %u + %u tokens > max_seq %u", seqs[i], m->seqs[seqs[i]].len,
+                             counts ? counts[i] : 1u, m->cfg.max_seq);
+    for (size_t i = 0; i < n; ++i)
+        if (int rc = drop_draft(m, seqs[i], counts ? counts[i] : 1u))
+            return rc;
     for (size_t i = 0; i < n; ++i)
         if (int rc = reserve(m, seqs[i], counts ? counts[i] : 1u))
         {

@@ -48,3 +48,50 @@ def test_drafts_of_many_calls_are_accepted_in_one(monkeypatch):
         want = _run(om, prompts[i] + [drafts[i][j] for j in keep[i]] + [7 + i])
         assert _rel_err(logits[i], want) < 1e-4, i
     bm.close()
+
+
+def test_a_dropped_draft_gives_its_pages_back(monkeypatch):
+    """Any call that drops a draft keeps the pages of the sequence's tokens and
+    of the call's own rows only."""
+    bm, om = _small_rows(monkeypatch, 256, 3)
+    total, free0 = bm.kv_pages()
+    s = bm.open()
+    p = _tokens(GQA, 260, 60)
+    bm.prefill(s, p)
+
+    def held():
+        return free0 - bm.kv_pages()[1]
+
+    def draft():
+        bm.step_tree([s], [_tokens(GQA, 261, 200)], [[-1] * 200], want_logits=False)
+        assert held() == 5
+
+    draft()
+    lg, _ = bm.step([s], [3])
+    assert held() == 1 and _rel_err(lg[0], _run(om, p + [3])) < 1e-4
+    draft()
+    lg, _ = bm.prefill_batch([s], [[4, 5, 6, 7]])
+    assert held() == 2 and _rel_err(lg[0], _run(om, p + [3, 4, 5, 6, 7])) < 1e-4
+    draft()
+    bm.step_tree([s], [[1, 2]], [[-1, 0]], want_logits=False)  # a smaller draft in its place
+    assert held() == 2
+    draft()
+    lg, _ = bm.prefill(s, [8])
+    assert held() == 2 and _rel_err(lg, _run(om, p + [3, 4, 5, 6, 7, 8])) < 1e-4
+    # the pages are another sequence's at once
+    draft()
+    o = bm.open()
+    bm.step([s], [9])
+    bm.prefill(o, _tokens(GQA, 262, 64 * (total - 2)))
+    assert bm.kv_pages()[1] == 0
+    lg, _ = bm.step([s], [10])
+    assert _rel_err(lg[0], _run(om, p + [3, 4, 5, 6, 7, 8, 9, 10])) < 1e-4
+    # two sequences of one call: the first may need what the second's draft held
+    bm.close_seq(o)
+    bm.step_tree([s], [[1] * 200], [[-1] * 200], want_logits=False)
+    o = bm.open()
+    bm.prefill(o, _tokens(GQA, 263, 64 * bm.kv_pages()[1]))
+    assert bm.kv_pages()[1] == 0
+    bm.step([o, s], [1, 2])
+    assert bm.kv_pages()[1] == 2
+    bm.close()
