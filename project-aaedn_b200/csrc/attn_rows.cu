@@ -2,6 +2,7 @@
 // (the sequences of a batch in one call), causal or under a tree mask, and
 // its C ABI.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -16,9 +17,16 @@ namespace aaedn_dev
 // Set when a bounded wait of a call without its own error word ran out (an
 // array of the module: no allocation, so a first call can be captured).
 __device__ unsigned g_attn_rows_err;
+static std::atomic<uint64_t> g_attn_rows_used{0}; // devices (bits) with such a call
 
 int attn_rows_err_check()
 {
+    int dev = 0;
+    if (!g_attn_rows_used.load(std::memory_order_acquire))
+        return AAEDN_OK; // no call yet: nothing to read back
+    AAEDN_CUDA_TRY(cudaGetDevice(&dev));
+    if (!(g_attn_rows_used.load(std::memory_order_acquire) >> (dev & 63) & 1u))
+        return AAEDN_OK;
     unsigned e = 0;
     AAEDN_CUDA_TRY(cudaMemcpyFromSymbol(&e, g_attn_rows_err, sizeof e));
     if (!e)
@@ -286,6 +294,9 @@ static int rows_err_word(const AttnRowsArgs& a, unsigned** err)
         void* p = nullptr;
         AAEDN_CUDA_TRY(cudaGetSymbolAddress(&p, g_attn_rows_err));
         *err = static_cast<unsigned*>(p);
+        int dev = 0;
+        AAEDN_CUDA_TRY(cudaGetDevice(&dev));
+        g_attn_rows_used.fetch_or(1ull << (dev & 63), std::memory_order_release);
     }
     return AAEDN_OK;
 }

@@ -95,3 +95,38 @@ def test_a_dropped_draft_gives_its_pages_back(monkeypatch):
     bm.step([o, s], [1, 2])
     assert bm.kv_pages()[1] == 2
     bm.close()
+
+
+QUIET_SYNC = """
+import sys, time
+sys.path[:0] = {paths!r}
+import torch
+import aaedn_b200 as ab
+torch.zeros(1, device="cuda")
+L = ab.lib()
+
+def least(call):
+    call()
+    took = []
+    for _ in range(30):
+        t = time.perf_counter()
+        for _ in range(50):
+            call()
+        took.append(time.perf_counter() - t)
+    return min(took) / 50
+
+a, b = least(lambda: L.aaedn_stream_sync(None)), least(lambda: L.aaedn_device_sync())
+print("stream %.2f us, device %.2f us" % (a * 1e6, b * 1e6))
+assert b < 2 * a + 2e-6
+"""
+
+
+def test_a_device_sync_reads_nothing_back_before_the_first_attention_call():
+    """A wait for an idle device takes about a microsecond, a word copied from it
+    about ten: in a program without packed or tree attention there is none."""
+    import os
+    import subprocess
+    import sys
+    paths = [os.path.dirname(os.path.dirname(os.path.abspath(ab.__file__)))]
+    r = subprocess.run([sys.executable, "-c", QUIET_SYNC.format(paths=paths)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
