@@ -79,32 +79,21 @@ constexpr uint32_t RT_Q_ROW = RT_HDP * 4u + 16u; // a query row in shared memory
 constexpr size_t RT_SMEM = (size_t)RT_NS * RT_STAGE + 128 * RT_Q_ROW + 1024; // + alignment slack
 
 // ---- the split of the work ----------------------------------------------------
-// sum over i < n of floor((a i + b) / 64)
-__host__ __device__ inline unsigned long long rt_floor_sum(unsigned long long n, unsigned long long a,
-                                                           unsigned long long b)
+// sum over i < n of floor((a i + b) / 64), 0 < a: the numerators' sum less that of
+// their remainders. Those repeat with the period 64 / g, g = gcd(a, 64), and are
+// over one period b mod g plus each multiple of g below 64; what n leaves of a
+// period is summed term by term.
+__host__ __device__ inline unsigned long long rt_floor_sum(unsigned long long n, unsigned a, unsigned long long b)
 {
-    unsigned long long m = 64, r = 0;
-    while (true)
+    const unsigned low = a & (0u - a), g = low < 64u ? low : 64u, period = 64u / g;
+    unsigned long long rest = n / period * (unsigned long long)(period * ((unsigned)b & (g - 1u)) + g * (period * (period - 1u) / 2u));
+    unsigned r = (unsigned)b & 63u;
+    for (unsigned i = (unsigned)n & (period - 1u); i > 0; --i)
     {
-        if (a >= m)
-        {
-            r += n * (n - 1) / 2 * (a / m);
-            a %= m;
-        }
-        if (b >= m)
-        {
-            r += n * (b / m);
-            b %= m;
-        }
-        const unsigned long long y = a * n + b;
-        if (y < m)
-            return r;
-        n = y / m;
-        b = y % m;
-        const unsigned long long t = m;
-        m = a;
-        a = t;
+        rest += r;
+        r = (r + a) & 63u;
     }
+    return (a * (n * (n - 1) / 2) + b * n - rest) / 64;
 }
 
 struct RtSeq
