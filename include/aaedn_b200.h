@@ -235,9 +235,11 @@ typedef struct {
  * d_row_start); its row r is the token in cache slot d_past[s] + r, whose K
  * and V are in the cache already, and attends slots 0 .. d_past[s] + r. Query
  * head h reads K/V head h / (n_heads / n_kv_heads). out = softmax(scale *
- * q k^T) v with the softmax and all sums in fp32; the products are fp32
- * accurate (2^-22 of each factor and 2^-38 of the largest K or V value of the
- * same page and head). Rows that no sequence owns keep their contents. Keys
+ * q k^T) v with the softmax and all sums in fp32. The products' factors are held
+ * to 2^-22 of each and 2^-38 of the largest value of the query row, or of the K
+ * or V values of the same page and head (above head_dim 128 in fp32). Scores and
+ * values may have any size that fp32 holds. Rows that no sequence owns keep their
+ * contents. Keys
  * in pages outside 0 .. n_pages - 1 or behind the table are left out; a row
  * with no key left gives zeros; NaN and infinities in slots that a row does
  * not attend have no effect on it, and a row that attends one is NaN.
@@ -247,7 +249,8 @@ typedef struct {
  * AAEDN_ATTN_ROWS_WORKSPACE_BYTES of scratch, which needs no
  * initialisation and holds nothing between calls; calls (and captured graphs)
  * that can overlap on the GPU need one each. A bounded device wait that ran
- * out is reported by aaedn_device_sync. */
+ * out is reported by the next aaedn_device_sync on that device, whichever
+ * caller's it was. */
 #define AAEDN_ATTN_ROWS_WORKSPACE_BYTES (32u << 20)
 int aaedn_cu_attention_packed(const float* d_q, size_t ldq, const aaedn_kv_cache* cache, const int32_t* d_row_start,
                               const int32_t* d_past, size_t n_seqs, size_t rows, size_t n_heads, float scale,
@@ -287,8 +290,9 @@ int aaedn_cu_kv_compact(float* const* h_arrays, size_t n_arrays, uint32_t n_page
 
 /* Next tokens of many rows of logits ([rows][ld], vocab of each used, vocab up
  * to 1000000): aaedn_cu_sample's order of the vocabulary (logit descending,
- * ties by the lower id) with top-k and min-p, per-row parameters and fp64
- * probabilities. With p_i = exp((l_i - max) / T), the kept tokens are the
+ * ties by the lower id) with top-k and min-p, per-row parameters and
+ * probabilities computed in fp64 and held in steps of 2^-44 of the largest
+ * (one below 2^-45 of it counts as 0). With p_i = exp((l_i - max) / T), the kept tokens are the
  * first top_k of the order, of those the ones with p_i >= min_p (so min_p is
  * relative to the most likely token), of those up to and including the first
  * whose cumulative mass reaches top_p times their mass; the token is the first
@@ -531,7 +535,8 @@ int aaedn_seq_prefill_batch(aaedn_model* m, const uint32_t* h_seqs, const uint32
  * (aaedn_cu_attention_tree). h_logits [nodes][vocab] and h_next [nodes]
  * (either may be null) receive what follows each node. The sequences keep
  * their lengths; aaedn_seq_accept then takes the nodes to keep. Any other
- * call on a sequence drops its draft. Synchronises. */
+ * call that adds tokens to a sequence, forks or closes it drops its draft and
+ * the pages of that. Synchronises. */
 int aaedn_model_step_tree(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts, const uint32_t* h_tokens,
                           const int32_t* h_parents, size_t n, const aaedn_sampling* sampling, float* h_logits,
                           uint32_t* h_next);
@@ -539,7 +544,8 @@ int aaedn_model_step_tree(aaedn_model* m, const uint32_t* h_seqs, const uint32_t
  * drafted tree listed in h_nodes (concatenated): a path from the sequence's
  * last token, every node the child of the one before. Their K/V rows move to
  * the sequence's next slots (aaedn_cu_kv_compact) and the rest of the draft is
- * dropped, its pages given back. AAEDN_ESTATE without a drafted tree. */
+ * dropped, its pages given back. Drafts of several aaedn_model_step_tree calls
+ * can be taken in one. AAEDN_ESTATE without a drafted tree. */
 int aaedn_seq_accept(aaedn_model* m, const uint32_t* h_seqs, const uint32_t* h_counts, const uint32_t* h_nodes,
                      size_t n);
 

@@ -73,9 +73,9 @@ namespace aaedn_dev
 // zeros in shared memory and noted: a row that attends it becomes NaN, the
 // others never multiply it. A row with no key gives zeros. Bound by the tiles'
 // loads and barriers (8 us a tile where an SM has one CTA): 1077 rows, 16
-// heads of 256 dims 0.77 ms, eight trees of 16 over 900, 32 heads 0.44 ms; by a
+// heads of 256 dims 0.78 ms, eight trees of 16 over 900, 32 heads 0.45 ms; by a
 // warp a row that reads its keys for itself 2.9 and 1.3 ms (only single rows
-// over short caches, 64 over 200 keys, were faster that way: 0.29 against 0.56).
+// over short caches, 64 over 200 keys, were faster that way: 0.29 against 0.57).
 // ---------------------------------------------------------------------------
 constexpr int RL_ROWS = 32, RL_KEYS = 32, RL_WARPS = 8, RL_RW = RL_ROWS / RL_WARPS, RL_LD = 256 + 4;
 constexpr size_t RL_SMEM = (size_t)(RL_ROWS + 2 * RL_KEYS) * RL_LD * 4;
@@ -397,7 +397,8 @@ static int rows_tc_launch(const AttnRowsArgs& a, cudaStream_t st)
 // dims wide, and half of each MMA would be padding (prompt of 2048 tokens 123
 // us, by the pairs 131; a tree of 16 over 4001 tokens 26, by the pairs 34).
 // 65..128 the pairs (a prompt of 4096 tokens, 64 heads over 8: 924 us when they
-// came, by single SMs 1053; eight sequences of 4120 tokens 259 and 274).
+// came, by single SMs 1053; eight sequences of 4120 tokens 259 and 274). Both as
+// measured when the choice was made.
 // Above, a tile's operands and sums do not fit one SM's tensor memory: fp32 on
 // the FMA units. (Where both run, one warp a row, the simplest kernel, was 70 to
 // 90 times slower than the tensor cores on prompts: 13.6 against 0.15 ms.)

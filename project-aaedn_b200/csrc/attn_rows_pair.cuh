@@ -16,16 +16,18 @@
 // The first CTA's warp 1 issues the MMAs of both; its barriers count the
 // arrivals of both CTAs, and its commits arrive on both CTAs' barriers.
 //
-// On a B200: one prompt of 4096 tokens, 64 query heads over 8, 800 us (three
+// On a B200, calls in a burst (at the 1000 W limit the long ones take up to 15 %
+// more): one prompt of 4096 tokens, 64 query heads over 8, 823 us (three
 // MMAs of full rate a product would be 490, one 163); eight sequences of 4120
-// new tokens in all, 32 heads over 8, 196 us; 2048 tokens, 32 heads, 147 us; a
+// new tokens in all, 32 heads over 8, 197 us; 2048 tokens, 32 heads, 149 us; a
 // tree of 16 nodes over 4001 cached tokens, 32 heads over 8, 34 us; sixteen
-// trees of 1 to 63 nodes over 0 to 4032, 64 heads, 134 us. A unit takes about
+// trees of 1 to 63 nodes over 0 to 4032, 64 heads, 135 us. A unit takes about
 // 3000 clocks, its MMAs 1536: P V waits for the weights of both CTAs, the
 // output sums for P V, the next P V for them, and softmax and each conversion,
 // one warp a scheduler, take about 2500 clocks of latencies a unit themselves
-// (the ragged case: tensor pipe 41 % active, issue slots 49 %, HBM 13 %). With all of that arithmetic cut out the
-// handshakes and MMAs alone take 573 us of the 800. Tried and slower: two units
+// (the ragged case: tensor pipe 40 % active, issue slots 49 %, HBM 13 %). With all
+// of that arithmetic cut out the handshakes and MMAs alone took 573 us of what
+// was 800 then. Tried and slower, from that 800: two units
 // as one group through softmax, P V and sums (844 us: the conversions spill),
 // the maximum kept from earlier units instead of a first pass over the scores
 // (836), 64 scores in registers (900), one more pair of score buffers in the

@@ -12,8 +12,8 @@
 // Precision: the cache is fp32, the MMA takes 16-bit factors. A factor x is
 // carried as x_hi + x_lo, both fp16, of x scaled by a power of two (q: per
 // row, K and V: per unit, P: by 2^14) that puts the largest magnitude at
-// 2^14..2^15: 22 significant bits for magnitudes down to 2^-28 of the
-// largest, an absolute 2^-39 of it below. Each product is three MMAs (hi lo,
+// 2^14..2^15: 22 significant bits for magnitudes down to 2^-17 of the
+// largest, an absolute 2^-39 of it below (the low part is then subnormal). Each product is three MMAs (hi lo,
 // lo hi, hi hi; lo lo is below 2^-22 of it), the small ones first, so that
 // the tensor core's rounding of its accumulator (up to one unit per MMA)
 // only counts for the hi hi ones. bf16 would need six products for this, and
@@ -46,10 +46,10 @@
 // reach the other rows of the tile through 0 * NaN.
 //
 // Bound by the conversion of K and V and by the ways between the roles, not by
-// the MMAs. On a B200 at head_dim 64 (32 query heads over 8): a prompt of 2048
-// tokens 123 us, eight prompts of 4120 tokens together 174 us, a tree of 16
-// over 4001 cached tokens 26 us; four short sequences at head_dim 48 24 us, of
-// which 16 us are the call's two launches.
+// the MMAs. On a B200 at head_dim 64 (32 query heads over 8), calls in a burst: a
+// prompt of 2048 tokens 121 us, eight prompts of 4120 tokens together 174 us, a
+// tree of 16 over 4001 cached tokens 27 us; four short sequences at head_dim 48
+// 23 us, of which 16 us are the call's two launches.
 #pragma once
 
 #include "attn_rows.h"
@@ -578,8 +578,7 @@ __device__ __forceinline__ float2 rt_weights(const float (&s)[16], float f, floa
 // Offsets above this are far: 14 - top and s f + off are then no longer both near
 // the exact value (spacings of 1/8 and more in exp2's argument; at 2^25 the weights
 // would leave the range of fp16), so a far offset is the sum of two floats. That
-// costs 2 % where no row is far, the vote on it: one prompt of 2048 tokens, 32
-// heads, 148 us from 145, a tree batch 134.4 from 133.9.
+// costs 1.5 % of long prompts, the vote on it; trees are equal.
 constexpr float RT_FAR = 1048576.0f;
 __device__ __forceinline__ bool rt_far(float off) { return fabsf(off) > RT_FAR && off < INFINITY; }
 
@@ -1296,7 +1295,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
 // ---------------------------------------------------------------------------
 // Joins the partial means of the tiles that a share's end went through: CTA
 // (boundary c, 8 rows), one row a warp. The tile's shares are taken in order.
-// At most two slots a CTA, 38 MB in all, from L2 behind two dependent loads:
+// At most two slots a CTA, 20 MB in all, from L2 behind two dependent loads:
 // 13 us after eight sequences of 4120 tokens, by itself and from cold caches.
 // ---------------------------------------------------------------------------
 constexpr int RJ_WARPS = 8;

@@ -1081,7 +1081,7 @@ static int device_status(aaedn_model* m)
         AAEDN_CUDA_TRY(cudaMemcpyAsync(w + 1, m->pf_err, 4, cudaMemcpyDeviceToHost, m->stream));
     AAEDN_CUDA_TRY(cudaStreamSynchronize(m->stream));
     if (m->pf_err && w[1] != 0u && *w == 0u)
-        return set_error(AAEDN_ETIMEOUT, "a bounded wait of a prefill GEMM ran out");
+        return set_error(AAEDN_ETIMEOUT, "a bounded wait of a prefill GEMM or of a packed or tree attention ran out");
     switch (*w)
     {
     case 0: return AAEDN_OK;

@@ -147,8 +147,8 @@ __device__ __forceinline__ int sr_fixed_bin(float l)
 // IEEE floating-point arithmetic", 1989): (l - M) / T = (k + r) ln2 / 128 with
 // |r| <= 1/2, exp = 2^(k / 128) exp(r ln2 / 128), the polynomial to r^4 (its
 // next term is 1.2e-15, the rounding of per_t 33 * 2^-53: within 2^-47). l - M
-// is exact, so the largest logit has exactly 2^44 units. The fp64 rate bounds
-// the passes that need masses: ten fp64 instructions a token.
+// is exact, so the largest logit has exactly 2^44 units. Ten fp64
+// instructions a token (256 rows 142 us, with a shorter table and two more 149).
 __device__ __forceinline__ uint64_t sr_mass(float l, const SrRow& r, const double* tbl)
 {
     if (!(r.M - l <= r.far))
@@ -348,10 +348,12 @@ __device__ __forceinline__ void sr_sort(SrShared& s, uint32_t n)
     __syncthreads();
 }
 
-// Bound by latencies (the cluster's barriers between a dozen passes) and, for
-// rows without top-k, by their masses in fp64: one row of 32000 12 us, 32 rows
-// of 128256 38 us, 256 rows 142 us (20 would be one read of the logits). A row
-// with top_k 50 takes 17 us of its cluster, one without top-k 25 to 35.
+// Bound by the passes over the slice (a row without top-k reads it four times)
+// and the cluster's barriers between them, not by the masses: 256 rows keep the
+// issue slots 68 % and the fp64 pipe 7 % active. In a burst one row of 32000
+// takes 12 us, 32 rows of 128256 39 us, 256 rows 140 us (20 would be one read of
+// the logits). A row with top_k 50 takes 17 us of its cluster, one without top-k
+// 25 to 35.
 // C CTAs a row; RES: the slice's logits stay in shared memory, else every pass
 // reads them again (from L2 after the first).
 template <int C, bool RES>
@@ -750,7 +752,7 @@ int sample_rows(const SampleRowsArgs& a, cudaStream_t st)
 {
     // The fewest CTAs a row whose shared memory holds it, then more while the
     // rows leave SMs idle and a CTA has over 2048 tokens. Measured at a
-    // vocabulary of 128256 (an earlier step, 32 rows now 38): 8 rows by 4 CTAs
+    // vocabulary of 128256 (an earlier step, 32 rows now 39): 8 rows by 4 CTAs
     // each 39 us, by 8 33; 32 rows by 4 41, by 8 63; 256 rows by 4 198, by 8
     // 386 (each CTA's passes cost their barriers and histogram whatever its
     // slice).

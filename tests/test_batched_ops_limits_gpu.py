@@ -137,3 +137,26 @@ def test_values_near_the_ends_of_their_range(hd, size):
 @pytest.mark.parametrize("size", [1e-33, 1e34, 5e37])
 def test_wide_heads_values_near_the_ends_of_their_range(hd, size):
     test_values_near_the_ends_of_their_range(hd, size)
+
+
+@pytest.mark.parametrize("hd", [48, 64, 128])
+def test_factors_of_very_different_sizes_stay_within_the_stated_bound(hd):
+    """K rows and dims of q that differ by up to 10^9 within a page and a row. What
+    the parts of a factor cannot hold next to the largest one counts: 2^-38 of
+    the largest K of the page times |q|, and of the largest q of the row times
+    |k|, moves a score by up to scale * hd * 2^-38 * kmax * qmax each; a weight by
+    twice that, and so the output (ref.attention's argument) by twice that of
+    the mean of |v| again."""
+    c = ref.Case(4, 2, hd, [60, 3], [100, 130], seed=hd)
+    rng = np.random.default_rng(hd)
+    with np.errstate(invalid="ignore"):
+        c.k *= np.float32(10.0) ** rng.integers(-9, 1, (c.n_pages, 1, 64, 1)).astype(np.float32)
+    c.q = (c.q.reshape(c.T, 4, hd) * np.float32(10.0) ** rng.integers(-9, 1, (c.T, 4, hd)).astype(np.float32)).reshape(c.T, -1)
+    got = _call(c, "packed")
+    want, tol = ref.attention("packed", c.q, c.k, c.v, c.table, c.start, c.past, c.H, c.scale)
+    vabs, _ = ref.attention("packed", c.q, c.k, np.abs(c.v), c.table, c.start, c.past, c.H, c.scale)
+    kmax = np.abs(c.k[np.isfinite(c.k)]).max()
+    qmax = np.abs(c.q).reshape(c.T, 4, hd).max(2).repeat(hd, axis=1)
+    tol = tol + 2 * (2 * 2 * c.scale * hd * 2.0 ** -38 * kmax * qmax) * vabs
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (bad.mean(), np.argwhere(bad)[:3])
