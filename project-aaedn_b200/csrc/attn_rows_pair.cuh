@@ -464,6 +464,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                         use = r.y;
                         fa = fb = 1.0f;
                     }
+                    __syncwarp(); // together into the loads
                 }
                 corr = rt_exp2(corr); // 0 before the first key
                 off = noff;
@@ -501,7 +502,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
         RtCursor<TREE> c;
         for (bool more = c.start(a, st0, share, R2); more && ok; more = c.next(a, R2), ++item)
         {
-            float acc[W]; // in units of `unit`, the largest scale of V so far
+            float acc[W]; // in units of `unit`, the largest scale of V that counts so far
 #pragma unroll
             for (int d = 0; d < W; ++d)
                 acc[d] = 0.0f;
@@ -531,20 +532,22 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
                     bad |= (sm.seen[g & 3u][i] & ((uint64_t)bad0 | (uint64_t)bad1 << 32)) != 0ull;
                 if (u + 1 == c.u1)
                     stat = sm.stats[item & 3u][i];
-                const float f = in[half].down; // a power of two, the same for all rows
-                if (f > unit)
-                {
-                    corr *= unit / f; // exact, or an underflow of sums that no longer count
-                    unit = f;
-                }
+                const float f = in[half].down; // a power of two
+                // exact, or an underflow of sums that no longer count; where the sums so far
+                // count nothing, neither does their scale. By selects, and a vote: the loads
+                // from tensor memory below are the whole warp's together.
+                const bool over = f > unit, none = corr == 0.0f;
+                corr = over ? corr * rt_ratio(unit, f) : corr;
+                unit = over || none ? f : unit;
                 const float2 c2 = make_float2(corr, corr);
-                const float down = f / unit;
+                const float down = rt_ratio(f, unit);
+                const bool scaled = __any_sync(0xffffffffu, down != 1.0f);
 #pragma unroll
                 for (int d0 = 0; d0 < W; d0 += 16)
                 {
                     float t[16];
                     rt_ld<16>(t_o + d0, t);
-                    if (down != 1.0f)
+                    if (scaled)
 #pragma unroll
                         for (int d = 0; d < 16; ++d)
                             t[d] *= down;

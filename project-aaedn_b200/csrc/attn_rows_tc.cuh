@@ -457,6 +457,13 @@ __device__ __forceinline__ void rt_scale_of(uint32_t max_bits, float& up, float&
     down = __uint_as_float((uint32_t)(127 - k) << 23);
 }
 
+// a / b of two powers of two, a <= b (a 0: some power of two)
+__device__ __forceinline__ float rt_ratio(float a, float b)
+{
+    const int d = (int)(__float_as_uint(b) >> 23) - (int)(__float_as_uint(a) >> 23);
+    return d > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - d) << 23);
+}
+
 template <int REGS>
 __device__ __forceinline__ void rt_regs_inc()
 {
@@ -609,6 +616,7 @@ __device__ __noinline__ float2 rt_far_unit(uint32_t ts, uint64_t seen, float fa,
     float now = 0.0f;
     if (use != 0.0f)
         *lo = now = fminf(use == off ? old : INFINITY, 14.0f - top);
+    __syncwarp();
     return make_float2(now - old, now);
 }
 
@@ -947,6 +955,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                         use = r.y;
                         f = 1.0f;
                     }
+                    __syncwarp(); // together into the loads
                 }
                 corr = rt_exp2(corr); // 0 before the first key
                 off = noff;
@@ -984,7 +993,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
         RtCursor<TREE> c;
         for (bool more = c.start(a, st0, share, R); more && ok; more = c.next(a, R), ++item)
         {
-            float acc[W]; // in units of `unit`, the largest scale of V so far
+            float acc[W]; // in units of `unit`, the largest scale of V that counts so far
 #pragma unroll
             for (int d = 0; d < W; ++d)
                 acc[d] = 0.0f;
@@ -1005,20 +1014,22 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attn_rows_tc_kernel(const AttnR
                     bad |= (sm.seen[g & 3u][i] & ((uint64_t)in.vbad[0] | (uint64_t)in.vbad[1] << 32)) != 0ull;
                 if (u + 1 == c.u1)
                     stat = sm.stats[item & 3u][i];
-                const float f = in.v_down; // a power of two, the same for all rows
-                if (f > unit)
-                {
-                    corr *= unit / f; // exact, or an underflow of sums that no longer count
-                    unit = f;
-                }
+                const float f = in.v_down; // a power of two
+                // exact, or an underflow of sums that no longer count; where the sums so far
+                // count nothing, neither does their scale. By selects, and a vote: the loads
+                // from tensor memory below are the whole warp's together.
+                const bool over = f > unit, none = corr == 0.0f;
+                corr = over ? corr * rt_ratio(unit, f) : corr;
+                unit = over || none ? f : unit;
                 const float2 c2 = make_float2(corr, corr);
-                const float down = f / unit;
+                const float down = rt_ratio(f, unit);
+                const bool scaled = __any_sync(0xffffffffu, down != 1.0f);
 #pragma unroll
                 for (int d0 = 0; d0 < W; d0 += 16)
                 {
                     float t[16];
                     rt_ld<16>(t_o + d0, t);
-                    if (down != 1.0f)
+                    if (scaled)
 #pragma unroll
                         for (int d = 0; d < 16; ++d)
                             t[d] *= down;

@@ -160,3 +160,21 @@ def test_factors_of_very_different_sizes_stay_within_the_stated_bound(hd):
     tol = tol + 2 * (2 * 2 * c.scale * hd * 2.0 ** -38 * kmax * qmax) * vabs
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (bad.mean(), np.argwhere(bad)[:3])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 160])
+def test_values_next_to_much_larger_ones_that_weigh_nothing(hd):
+    """The first page holds values of 1e38 whose weights are exactly 0 (scores more
+    than 1000 below the others'), the pages behind it values of 1e-32: the result
+    is that of the pages behind it alone."""
+    S = 400  # so that a share of the work has all pages of a sequence
+    c = ref.Case(4, 2, hd, [1 + i % 2 for i in range(S)], [150] * S, seed=hd)
+    first = c.table[:, 0].copy()
+    with np.errstate(invalid="ignore"):
+        c.v *= np.float32(1e-32)
+    c.v[first] = np.float32(1e38) * np.sign(np.random.default_rng(1).normal(size=c.v[first].shape)).astype(np.float32)
+    c.q[:] = np.abs(c.q) + 1.0
+    c.k[first] = -40.0 * np.sqrt(hd)
+    got = _call(c, "packed")
+    c.table[:, 0] = -1  # left out
+    _check_scaled(c, "packed", got)
