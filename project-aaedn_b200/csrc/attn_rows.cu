@@ -73,7 +73,7 @@ namespace aaedn_dev
 // zeros in shared memory and noted: a row that attends it becomes NaN, the
 // others never multiply it. A row with no key gives zeros. Bound by the tiles'
 // loads and barriers (8 us a tile where an SM has one CTA): 1077 rows, 16
-// heads of 256 dims 0.78 ms, eight trees of 16 over 900, 32 heads 0.45 ms; by a
+// heads of 256 dims 0.79 ms, eight trees of 16 over 900, 32 heads 0.46 ms; by a
 // warp a row that reads its keys for itself 2.9 and 1.3 ms (only single rows
 // over short caches, 64 over 200 keys, were faster that way: 0.29 against 0.57).
 // ---------------------------------------------------------------------------

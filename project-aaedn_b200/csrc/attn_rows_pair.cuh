@@ -17,11 +17,11 @@
 // arrivals of both CTAs, and its commits arrive on both CTAs' barriers.
 //
 // On a B200, calls in a burst (at the 1000 W limit the long ones take up to 15 %
-// more): one prompt of 4096 tokens, 64 query heads over 8, 823 us (three
+// more): one prompt of 4096 tokens, 64 query heads over 8, 816 us (three
 // MMAs of full rate a product would be 490, one 163); eight sequences of 4120
-// new tokens in all, 32 heads over 8, 197 us; 2048 tokens, 32 heads, 149 us; a
+// new tokens in all, 32 heads over 8, 198 us; 2048 tokens, 32 heads, 149 us; a
 // tree of 16 nodes over 4001 cached tokens, 32 heads over 8, 34 us; sixteen
-// trees of 1 to 63 nodes over 0 to 4032, 64 heads, 135 us. A unit takes about
+// trees of 1 to 63 nodes over 0 to 4032, 64 heads, 134 us. A unit takes about
 // 3000 clocks, its MMAs 1536: P V waits for the weights of both CTAs, the
 // output sums for P V, the next P V for them, and softmax and each conversion,
 // one warp a scheduler, take about 2500 clocks of latencies a unit themselves

@@ -47,7 +47,7 @@
 //
 // Bound by the conversion of K and V and by the ways between the roles, not by
 // the MMAs. On a B200 at head_dim 64 (32 query heads over 8), calls in a burst: a
-// prompt of 2048 tokens 121 us, eight prompts of 4120 tokens together 174 us, a
+// prompt of 2048 tokens 119 us, eight prompts of 4120 tokens together 174 us, a
 // tree of 16 over 4001 cached tokens 27 us; four short sequences at head_dim 48
 // 23 us, of which 16 us are the call's two launches.
 #pragma once
